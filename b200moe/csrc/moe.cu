@@ -3,7 +3,7 @@
 // with no host round trip), the row gather into the padded expert-major layout,
 // the weighted combine and their backward duals.
 //
-// Layout contract.  Slots are numbered s = 2*token + j.  Expert e owns rows
+// Layout contract.  Slots are numbered s = k*token + j, k experts per token (2 where nothing else is said).  Expert e owns rows
 // [seg_start[e], seg_start[e] + count[e]) of the permuted buffer, in slot order;
 // every segment is padded with zero rows to a multiple of 256 so a GEMM tile
 // never straddles two experts.  ``slot_row[s]`` is the row of slot s,
@@ -149,7 +149,7 @@ struct alignas(16) vec16 {
   uint32_t v[4];
 };
 
-// x_perm[r] = scale(slot) * x[slot / 2] for live rows, zeros for padding; one warp per row.
+// x_perm[r] = scale(slot) * x[slot / k] for live rows, zeros for padding; one warp per row.
 // ``scale`` is null (dispatch) or the per-slot routing weight (backward of combine).
 // With ``y_perm``/``dweights`` the kernel also emits dweights[slot] = <x[token], y_perm[r]>.
 __global__ void __launch_bounds__(256) moe_gather_kernel(const __nv_bfloat16* __restrict__ x,
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(const __nv_bfloat16* __
                                                          const __nv_bfloat16* __restrict__ y_perm,
                                                          float* __restrict__ dweights,
                                                          __nv_bfloat16* __restrict__ x_perm, int D, int capacity_rows,
-                                                         int slots) {
+                                                         int slots, int k) {
   chain_begin();
   const int live_rows = min(meta[1], capacity_rows);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(const __nv_bfloat16* __
       continue;
     }
     if (!dbg_in_range(slot, 0, slots, 411)) continue;
-    const __nv_bfloat16* src = x + static_cast<size_t>(slot >> 1) * D;
+    const __nv_bfloat16* src = x + static_cast<size_t>(k == 2 ? slot >> 1 : slot / k) * D;
     if (!scale) {
       for (int c = lane * 8; c < D; c += 256) *reinterpret_cast<vec16*>(dst + c) = *reinterpret_cast<const vec16*>(src + c);
       continue;
@@ -233,6 +233,50 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const __nv_bfloat16* _
           const float2 f = __bfloat1622float2(r);
           r = __floats2bfloat162_rn(fr.x + f.x, fr.y + f.y);
         }
+        o.v[i] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+      *reinterpret_cast<vec16*>(out + static_cast<size_t>(t) * D + c) = o;
+    }
+  }
+}
+
+// The same for k experts per token: out[t] = sum over j of w_j * y[slot_row[k t + j]], added in the order of j in fp32.  Bound by the
+// k rows that it reads; the loop over the experts is inside that over the columns, so a lane has its k loads in flight.
+__global__ void __launch_bounds__(256) moe_combine_k_kernel(const __nv_bfloat16* __restrict__ y_perm,
+                                                            const int* __restrict__ slot_row,
+                                                            const float* __restrict__ weights,
+                                                            __nv_bfloat16* __restrict__ out, int T, int D, int rows, int k) {
+  chain_begin();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int t = blockIdx.x * 8 + warp; t < T; t += gridDim.x * 8) {
+    const long long first = static_cast<long long>(t) * k;
+    // lane j holds the row and the weight of expert j (at most 32)
+    const int my_row = lane < k ? slot_row[first + lane] : 0;
+    const float my_weight = lane < k && weights ? weights[first + lane] : 1.f;
+    if (__any_sync(0xffffffffu, !dbg_in_range(my_row, 0, rows, 413))) continue;
+    for (int c0 = 0; c0 < D; c0 += 256) {
+      const int c = c0 + lane * 8;
+      float sum[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+#pragma unroll 4
+      for (int j = 0; j < k; ++j) {
+        const int r = __shfl_sync(0xffffffffu, my_row, j);
+        const float w = __shfl_sync(0xffffffffu, my_weight, j);
+        if (c >= D) continue;
+        const vec16 v = *reinterpret_cast<const vec16*>(y_perm + static_cast<size_t>(r) * D + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.v[i]));
+          sum[2 * i] = __fmaf_rn(w, f.x, sum[2 * i]);
+          sum[2 * i + 1] = __fmaf_rn(w, f.y, sum[2 * i + 1]);
+        }
+      }
+      if (c >= D) continue;
+      vec16 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(sum[2 * i], sum[2 * i + 1]);
         o.v[i] = *reinterpret_cast<const uint32_t*>(&r);
       }
       *reinterpret_cast<vec16*>(out + static_cast<size_t>(t) * D + c) = o;
@@ -409,9 +453,14 @@ extern "C" {
 int b2_moe_plan(const long long* idx, int slots, int E, int* slot_row, int* row_slot, int* offs, int* tile_expert,
                 int* meta, int* counts, int capacity_rows, cudaStream_t s) {
   if (E < 1) return -10;
-  // 49 experts are what an earlier form of the kernel held in shared memory; this one needs 144 bytes an expert.  The limit
-  // stays what callers and tests know.
-  if (E > 49) return -11;
+  if (E > 1024) return -11;                 // 144 bytes of shared memory an expert
+  if (E > 300) {
+    static bool set = false;
+    if (!set) {
+      if (cudaFuncSetAttribute(moe_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess) return -3;
+      set = true;
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -434,12 +483,18 @@ int b2_moe_plan(const long long* idx, int slots, int E, int* slot_row, int* row_
   return 0;
 }
 
+// ``k`` experts per token: slots = k * tokens.
+int b2_moe_gather_k(const void* x, const int* row_slot, const int* meta, const float* scale, const void* y_perm,
+                    float* dweights, void* x_perm, int D, int capacity_rows, int slots, int k, cudaStream_t s) {
+  if (D % 8 || k < 1) return -10;
+  launch_next(moe_gather_kernel, sm_count_moe() * 8, 256, 0, s, (const bf16*)x, row_slot, meta, scale, (const bf16*)y_perm,
+              dweights, (bf16*)x_perm, D, capacity_rows, slots, k);
+  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+}
+
 int b2_moe_gather(const void* x, const int* row_slot, const int* meta, const float* scale, const void* y_perm,
                   float* dweights, void* x_perm, int D, int capacity_rows, int slots, cudaStream_t s) {
-  if (D % 8) return -10;
-  launch_next(moe_gather_kernel, sm_count_moe() * 8, 256, 0, s, (const bf16*)x, row_slot, meta, scale, (const bf16*)y_perm,
-              dweights, (bf16*)x_perm, D, capacity_rows, slots);
-  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+  return b2_moe_gather_k(x, row_slot, meta, scale, y_perm, dweights, x_perm, D, capacity_rows, slots, 2, s);
 }
 
 int b2_moe_combine(const void* y_perm, const int* slot_row, const float* weights, const void* residual, void* out,
@@ -447,6 +502,15 @@ int b2_moe_combine(const void* y_perm, const int* slot_row, const float* weights
   if (D % 8) return -10;
   launch_next(moe_combine_kernel, min((T + 7) / 8, sm_count_moe() * 8), 256, 0, s, (const bf16*)y_perm, slot_row, weights,
               (const bf16*)residual, (bf16*)out, T, D, rows);
+  return cudaGetLastError() == cudaSuccess ? 0 : -1;
+}
+
+// k experts per token, at most 32; weights null: 1.
+int b2_moe_combine_k(const void* y_perm, const int* slot_row, const float* weights, void* out, int T, int D, int rows, int k,
+                     cudaStream_t s) {
+  if (D % 8 || k < 1 || k > 32) return -10;
+  launch_next(moe_combine_k_kernel, min((T + 7) / 8, sm_count_moe() * 8), 256, 0, s, (const bf16*)y_perm, slot_row, weights,
+              (bf16*)out, T, D, rows, k);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 

@@ -132,6 +132,14 @@ __device__ __forceinline__ void umma_bf16_ss(uint32_t tmem_d, uint64_t desc_a, u
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same with 8-bit floating point inputs (types in the instruction descriptor), 32 values along the reduction.
+__device__ __forceinline__ void umma_f8_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // A operand read from TMEM (bf16 packed), B from shared memory.
 __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
                                              uint32_t accumulate) {
@@ -256,9 +264,9 @@ __device__ __forceinline__ void fence_async_shared() {
 
 // ---------------------------------------------------------------- UMMA descriptors
 // Shared-memory operand descriptor, 128-byte swizzle.  ``lbo``/``sbo`` in bytes.
-//   K-major tile  (rows x 64 bf16, 128 B per row): sbo = 1024 (8-row group pitch), lbo unused.
+//   K-major tile  (rows x 64 bf16 or 128 8-bit values, 128 B per row): sbo = 1024 (8-row group pitch), lbo unused.
 //   MN-major tile (64 bf16 along MN per 128 B row, K rows): sbo = 1024 (8 K-rows), lbo = pitch
-//   between 64-element MN chunks.
+//   between 64-element MN chunks; 8-bit values: 128 along MN per row.
 __device__ __forceinline__ uint64_t umma_smem_desc(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
@@ -274,7 +282,12 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n, int a_mn_ma
          (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
-// The same with fp16 A/B.
+// Instruction descriptor for kind::f8f6f4 with e4m3 A (K-major) and B, fp32 D.
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n, int b_mn_major) {
+  return (1u << 4) | (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+// The same as umma_idesc_bf16 with fp16 A/B.
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, int a_mn_major, int b_mn_major) {
   return umma_idesc_bf16(m, n, a_mn_major, b_mn_major) & ~((1u << 7) | (1u << 10));
 }

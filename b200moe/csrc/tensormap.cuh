@@ -50,6 +50,20 @@ static inline int make_map(CUtensorMap* map, const void* base, long long inner, 
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
+// The same for 8-bit values: box = [box_outer, 128] bytes.  Base and pitch are multiples of 16 bytes.
+static inline int make_map8(CUtensorMap* map, const void* base, long long inner, long long outer, long long pitch, int box_outer) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+  cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_outer)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
 // fp32 result [experts, rows, cols] with row pitch ``pitch_elems`` and expert pitch ``expert_elems``, as the epilogue's
 // stores address it: boxes of 32 rows x 32 columns, 128B swizzle.
 static inline int make_out_map(CUtensorMap* map, const void* base, long long cols, long long rows, long long experts,

@@ -260,23 +260,39 @@ class PositionWiseFFLayer(nn.Module):
 class MoELayerMulti(nn.Module):
     """Top-2 routed experts partitioned over ``dp_group`` (reference
     layers.py:100-213).  ``compute dtype`` defaults to bf16; fp32 is accepted so
-    the CPU tier can be compared bit-tight against an fp32 oracle."""
+    the CPU tier can be compared bit-tight against an fp32 oracle.
+
+    ``routing``: keyword arguments of ``ops.route_topk`` (``score``, ``groups``, ``top_groups``, ``group_score``,
+    ``renormalize``, ``scale``; an empty dict takes its defaults) for another router than the softmax of two experts, with
+    any ``k`` that it takes; ``balance_bias: True`` adds the buffer ``expert_bias``, which takes part in the choice and which
+    the training loop moves against the experts' load.  On a GPU the router's product has up to 16 experts or a multiple
+    of 64."""
 
     def __init__(self, d_model, d_ff, k=2, num_expert_per_node=4, device=None, dtype=torch.bfloat16,
-                 dp_group=None):
+                 dp_group=None, routing=None):
         super().__init__()
         import torch.distributed as dist
         self.dp_group = dp_group
         self.world_size = 1 if dp_group is None else dist.get_world_size(dp_group)
         if num_expert_per_node < 1 or not 1 <= k <= self.world_size * num_expert_per_node:
             raise ValueError("Require positive expert count and 1 <= k <= total experts")
-        if k != 2:
+        if k != 2 and routing is None:
             raise ValueError("The fused router implements top-2 routing")
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("Grouped MoE requires torch.bfloat16 compute dtype (float32 on CPU)")
         self.dtype, self.k, self.num_expert_per_node = dtype, k, num_expert_per_node
         self.experts = GroupedPositionWiseFFLayer(num_expert_per_node, d_model, d_ff, device=device, dtype=dtype)
         self.router = LinearLayer(d_model, self.world_size * num_expert_per_node, device=device)
+        self.routing = None if routing is None else dict(routing)
+        biased = False
+        if self.routing is not None:
+            known = {"score", "groups", "top_groups", "group_score", "renormalize", "scale"}
+            biased = self.routing.pop("balance_bias", False)
+            if set(self.routing) - known:
+                raise ValueError(f"routing takes {sorted(known | {'balance_bias'})}, got {sorted(set(self.routing) - known)}")
+            experts_total = self.world_size * num_expert_per_node
+            ops.route_topk(torch.zeros(0, experts_total), k, **self.routing)          # refuses what does not fit
+        self.register_buffer("expert_bias", torch.zeros(self.world_size * num_expert_per_node, device=device) if biased else None)
         self.recompute = False
         self.budget = None  # parallel.memory.ActivationBudget of the stage (set by the trainer), or None
         self.comm = None  # peer-memory communication layer, set by the FSDP wrapper (fused backend)
@@ -285,10 +301,10 @@ class MoELayerMulti(nn.Module):
         return self._forward(x, return_aux_loss, None)
 
     def _one_op(self, x) -> bool:
-        """Whether router and experts run as one op: one rank, the kernels of every step switched on, and nobody watches
-        the router's calls."""
+        """Whether router and experts run as one op: the router of the standard block on one rank, the kernels of every step
+        switched on, and nobody watches the router's calls."""
         router = self._modules["router"]
-        return (self.world_size == 1 and ops.use_native(x, "moe") and ops.use_native(x, "router")
+        return (self.routing is None and self.world_size == 1 and ops.use_native(x, "moe") and ops.use_native(x, "router")
                 and ops.use_native(x, "gemm") and type(router) is LinearLayer
                 and type(self._modules["experts"]) is GroupedPositionWiseFFLayer and not _hooked(router))
 
@@ -321,7 +337,7 @@ class MoELayerMulti(nn.Module):
             return (out, aux) if return_aux_loss else out
         experts_total = self.world_size * self.num_expert_per_node
         ep_ctx = None
-        if self.comm is not None and self.world_size > 1 and flat.is_cuda:
+        if self.comm is not None and self.world_size > 1 and flat.is_cuda and self.routing is None:
             ep_ctx = self.comm.ep_context(flat.shape[0], flat.shape[1], experts_total, self.experts.dff)
         if ep_ctx is not None and ops.use_native(flat, "moe"):
             # exchange fused with the expert GEMMs: the router reads the staged copy of the input that the other
@@ -337,8 +353,13 @@ class MoELayerMulti(nn.Module):
                                              recompute=self.recompute, key=id(self), budget=self.budget)
             logits = seen["logits"]
         else:
+            if self.routing is not None and flat.is_cuda and experts_total > 16 and experts_total % 64:
+                raise ValueError(f"on a GPU the router has up to 16 experts or a multiple of 64, got {experts_total}")
             logits = self.router(flat)
-            weights, idx = ops.router_top2(logits)
+            if self.routing is None:
+                weights, idx = ops.router_top2(logits)
+            else:
+                weights, idx = ops.route_topk(logits, self.k, bias=self.expert_bias, **self.routing)
             out = ops.moe_ffn(flat, weights, idx, self.experts.w1, self.experts.w2, self.experts.w3,
                               group=self.dp_group if self.world_size > 1 else None,
                               recompute=self.recompute, budget=self.budget)

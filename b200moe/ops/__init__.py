@@ -60,13 +60,15 @@ def backward_follows(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-from .dense import linear, linear_rope, swiglu_ffn, embedding, rmsnorm, add_rmsnorm  # noqa: E402
+from .dense import linear, linear_rope, swiglu_ffn, embedding, rmsnorm, add_rmsnorm, gated_add_rmsnorm  # noqa: E402
 from .attention import rope_attention  # noqa: E402
 from .loss import lm_head_cross_entropy  # noqa: E402
-from .moe import router_top2, moe_ffn, DispatchPlan  # noqa: E402
+from .moe import router_top2, route_topk, moe_ffn, DispatchPlan  # noqa: E402
+from .fp8 import quantize_fp8, matmul_fp8, linear_fp8  # noqa: E402
 
 __all__ = [
     "Fn", "set_native", "native_enabled", "use_native", "backward_follows", "linear", "linear_rope", "swiglu_ffn",
-    "embedding", "rmsnorm", "add_rmsnorm",
-    "rope_attention", "lm_head_cross_entropy", "router_top2", "moe_ffn", "DispatchPlan",
+    "embedding", "rmsnorm", "add_rmsnorm", "gated_add_rmsnorm",
+    "rope_attention", "lm_head_cross_entropy", "router_top2", "route_topk", "moe_ffn", "DispatchPlan",
+    "quantize_fp8", "matmul_fp8", "linear_fp8",
 ]

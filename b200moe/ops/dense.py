@@ -11,7 +11,10 @@ Replaces the reference's ``einsum`` linear (implementation/layers.py:55-69),
 """
 from __future__ import annotations
 
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import backward_follows, cpp_nodes, functional as Fn, native, use_native
 
@@ -227,3 +230,82 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, eps:
         return _AddRMSNorm.apply(x, delta, weight, eps)
     summed = x + delta
     return summed, Fn.rmsnorm_ref(summed, weight, eps)
+
+
+_GATE_KINDS = ("none", "channel", "sequence", "token", "full")
+
+
+def _gate_kind(x, gate) -> int:
+    """Index into ``_GATE_KINDS``; what two kinds would take is the one with fewer values to add up."""
+    if gate is None:
+        return 0
+    shape, width = tuple(x.shape), x.shape[-1]
+    if gate.shape == x.shape:
+        return 4
+    if tuple(gate.shape) == (width,):
+        return 1
+    if tuple(gate.shape) == shape[:-1] + (1,):
+        return 3
+    if x.dim() >= 3 and tuple(gate.shape) == shape[:1] + (1,) * (x.dim() - 2) + (width,):
+        return 2
+    raise ValueError(f"a gate for x {shape} is [{width}], {list(shape[:1] + (1,) * (x.dim() - 2) + (width,))}, "
+                     f"{list(shape[:-1] + (1,))} or {list(shape)}, got {list(gate.shape)}")
+
+
+def _gated_add_rmsnorm(x, delta, delta_weight, weight, gate, kind, seq, residual_scale, eps):
+    """The kernel's outputs, and its operands as it read them."""
+    operands = (x.contiguous(), delta.contiguous(), delta_weight.float().contiguous(), weight.float().contiguous(),
+                None if gate is None else gate.contiguous())
+    return *native.gated_norm_fwd(*operands, kind, seq, residual_scale, eps), operands
+
+
+class _GatedAddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, delta, delta_weight, weight, gate, kind, seq, residual_scale, eps):
+        ctx.set_materialize_grads(False)
+        summed, normed, stats, operands = _gated_add_rmsnorm(x, delta, delta_weight, weight, gate, kind, seq, residual_scale, eps)
+        ctx.save_for_backward(*operands, stats)
+        ctx.how = (kind, seq, residual_scale)
+        ctx.types = (delta_weight.dtype, weight.dtype)
+        return summed, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dsummed, dnormed):
+        if dsummed is None and dnormed is None:
+            return (None,) * 9
+        grads = (None if g is None else g.contiguous() for g in (dsummed, dnormed))
+        dx, ddelta, dwd, dw, dgate = native.gated_norm_bwd(*grads, *ctx.saved_tensors, *ctx.how)
+        return dx, ddelta, dwd.to(ctx.types[0]), dw.to(ctx.types[1]), dgate, None, None, None, None
+
+
+def gated_add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, delta_weight: torch.Tensor, weight: torch.Tensor, *,
+                      gate: torch.Tensor | None = None, residual_scale: float = 1.0, eps: float = 1e-5):
+    """The seam between two blocks with norms on both sides: ``summed = residual_scale · x + gate · rmsnorm(delta,
+    delta_weight)`` and ``rmsnorm(summed, weight)``, the latter of the sum before it is rounded; returns both.
+
+    ``x`` and ``delta`` ``[..., D]`` have one type (bf16, fp16 or fp32; D up to 8192).  ``gate``, of that type or fp32, has
+    the shape ``[D]``, ``[B, 1, D]`` for ``x [B, S, D]``, ``[..., 1]`` or that of ``x``."""
+    if x.shape != delta.shape or x.dim() < 1:
+        raise ValueError(f"x {list(x.shape)} and delta {list(delta.shape)} must have one shape [..., D]")
+    width = x.shape[-1]
+    if delta_weight.shape != (width,) or weight.shape != (width,):
+        raise ValueError(f"the weights must be [{width}], got {list(delta_weight.shape)} and {list(weight.shape)}")
+    kind = _gate_kind(x, gate)
+    if x.dtype != delta.dtype or (gate is not None and gate.dtype not in (x.dtype, torch.float32)):
+        raise TypeError(f"x and delta must have one type, the gate that or fp32: got {x.dtype}, {delta.dtype}"
+                        f"{'' if gate is None else f', {gate.dtype}'}")
+    if not (math.isfinite(residual_scale) and eps > 0):
+        raise ValueError(f"residual_scale must be finite and eps positive, got {residual_scale} and {eps}")
+    for t in (delta, delta_weight, weight, gate):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"all tensors must be on {x.device}, got one on {t.device}")
+    if not use_native(x, "gated_norm"):
+        return Fn.gated_add_rmsnorm_ref(x, delta, delta_weight, weight, gate, residual_scale, eps)
+    if not 1 <= width <= 8192:
+        raise ValueError(f"rows of 1 to 8192 values, got {width}")
+    seq = x.numel() // max(x.shape[0] * width, 1) if kind == 2 else 1
+    args = (x, delta, delta_weight, weight, gate, kind, max(seq, 1), float(residual_scale), float(eps))
+    if backward_follows(x, delta, delta_weight, weight, gate):
+        return _GatedAddRMSNorm.apply(*args)
+    return _gated_add_rmsnorm(*args)[:2]

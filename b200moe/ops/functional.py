@@ -16,6 +16,7 @@ __all__ = [
     "softmax", "silu", "cross_entropy", "gradient_clipping", "gradient_clippling", "sample_output",
     "dot_product_att", "rmsnorm_ref", "rope_tables", "apply_rope_ref", "attention_ref",
     "router_top2_ref", "swiglu_ref", "grouped_mm_ref", "log_softmax", "clip_gradient",
+    "route_topk_ref", "gated_add_rmsnorm_ref", "quantize_fp8_ref", "dequantize_fp8_ref",
 ]
 
 
@@ -133,6 +134,111 @@ def router_top2_ref(logits: torch.Tensor, k: int = 2):
     probs = softmax(logits.float(), dim_sum=-1)
     top, idx = probs.topk(k, dim=-1)
     return top / top.sum(dim=-1, keepdim=True), idx
+
+
+def route_topk_ref(logits: torch.Tensor, k: int, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
+                   top_groups: int | None = None, group_score: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """``(weights fp32 [T, k], idx int64 [T, k])`` of ``logits [T, E]``.  Experts are chosen by their scores plus ``bias``
+    (without one: by their logits), best first, the lower index first where two are equal, after a choice of the
+    ``top_groups`` best of ``groups`` runs of experts by their best key or the sum of their two best.  The weights are the
+    scores without the bias.  NaN and -inf mask an expert: it is chosen after all others of its groups, with weight 0.
+    What decides the choice is evaluated in fp64."""
+    tokens, experts = logits.shape
+    top_groups = groups if top_groups is None else top_groups
+    wide = logits if logits.dtype == torch.float64 else logits.float()
+    x = torch.where(torch.isnan(wide), -math.inf, wide).clamp(max=torch.finfo(torch.float32).max)
+    dead = torch.isinf(x)
+
+    def scores(t, off):
+        """Scores of ``t``, zero where ``off``; what is masked takes no part in a gradient either."""
+        safe = t.masked_fill(off, 0.0)
+        if score == "sigmoid":
+            return torch.sigmoid(safe) * (~off).to(t.dtype)
+        top = t.detach().masked_fill(off, -math.inf).amax(-1, keepdim=True)
+        part = torch.exp(safe - top.masked_fill(torch.isinf(top), 0.0)).masked_fill(off, 0.0)
+        total = part.sum(-1, keepdim=True)
+        return part / torch.where(total == 0, torch.ones_like(total), total)
+
+    with torch.no_grad():
+        key = x.double()
+        grouped = top_groups < groups
+        compared = key
+        if bias is not None or (grouped and group_score == 2):
+            s = key
+            if score == "sigmoid":
+                s = 1.0 / (1.0 + torch.exp(-key))
+            else:
+                s = scores(key, dead)
+            compared = (s if bias is None else s + bias.double()).masked_fill(dead, -math.inf)
+            if bias is not None:
+                key = compared
+        level = torch.ones_like(key)
+        if grouped:
+            best = compared.view(tokens, groups, experts // groups).sort(-1, descending=True).values
+            value = best[..., 0]
+            if group_score == 2:
+                value = value + best[..., 1].masked_fill(torch.isinf(best[..., 1]), 0.0)
+            order = torch.sort(value, dim=-1, descending=True, stable=True).indices[:, :top_groups]
+            chosen = torch.zeros_like(value).scatter_(1, order, 1.0)
+            level = chosen.repeat_interleave(experts // groups, dim=1)
+        # experts of other groups last, masked ones of the chosen groups before them
+        rank = torch.sort(key, dim=-1, descending=True, stable=True).indices
+        rank = rank.gather(1, torch.sort(level.gather(1, rank), dim=-1, descending=True, stable=True).indices)
+        idx = rank[:, :k]
+    off = dead.gather(1, idx)
+    if renormalize:
+        picked = x.gather(1, idx).masked_fill(off, 0.0)
+        logs = F.logsigmoid(picked) if score == "sigmoid" else picked
+        top = logs.detach().masked_fill(off, -math.inf).amax(-1, keepdim=True)
+        part = torch.exp(logs - top.masked_fill(torch.isinf(top), 0.0)).masked_fill(off, 0.0)
+        total = part.sum(-1, keepdim=True)
+        weights = part / torch.where(total == 0, torch.ones_like(total), total)
+    else:
+        weights = scores(x, dead).gather(1, idx)
+    return weights * scale, idx
+
+
+def gated_add_rmsnorm_ref(x: torch.Tensor, delta: torch.Tensor, delta_weight: torch.Tensor, weight: torch.Tensor,
+                          gate: torch.Tensor | None = None, residual_scale: float = 1.0, eps: float = 1e-5):
+    """``s = residual_scale x + gate rmsnorm(delta) delta_weight`` and ``rmsnorm(s) weight``, in fp32 (fp64 stays); the second
+    norm sees the sum before it is rounded."""
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+
+    def norm(t):
+        return t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + eps)
+
+    branch = norm(delta.to(wide)) * delta_weight.to(wide)
+    if gate is not None:
+        branch = branch * gate.to(wide)
+    summed = x.to(wide) * residual_scale + branch
+    return summed.to(x.dtype), (norm(summed) * weight.to(wide)).to(x.dtype)
+
+
+E4M3_MAX = 448.0
+SMALLEST_FP8_SCALE = 2.0 ** -120
+
+
+def _fp8_blocks(x: torch.Tensor, block_rows: int) -> torch.Tensor:
+    x = F.pad(x.float(), (0, -x.shape[1] % 128, 0, -x.shape[0] % block_rows))
+    return x.view(x.shape[0] // block_rows, block_rows, x.shape[1] // 128, 128)
+
+
+def quantize_fp8_ref(x: torch.Tensor, block_rows: int = 1):
+    """e4m3 values of ``x [M, K]`` and one fp32 scale for each block of ``block_rows`` x 128 of them: ``max(largest / 448,
+    2^-120)``, so that the largest value becomes 448, the largest number of the type."""
+    rows, cols = x.shape
+    blocks = _fp8_blocks(x, block_rows)
+    most = torch.where(torch.isnan(blocks), 0.0, blocks.abs()).amax((1, 3))
+    scales = (most / E4M3_MAX).clamp(min=SMALLEST_FP8_SCALE)
+    values = (blocks / scales[:, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+    return values.view(blocks.shape[0] * block_rows, blocks.shape[2] * 128)[:rows, :cols].contiguous(), scales
+
+
+def dequantize_fp8_ref(values: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> torch.Tensor:
+    """The fp32 numbers that ``quantize_fp8`` stands for."""
+    rows, cols = values.shape
+    blocks = _fp8_blocks(values, block_rows) * scales[:, None, :, None]
+    return blocks.view(blocks.shape[0] * block_rows, blocks.shape[2] * 128)[:rows, :cols]
 
 
 def swiglu_ref(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:

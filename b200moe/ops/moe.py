@@ -18,13 +18,15 @@ tier and the NCCL A/B baseline.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
 import torch.distributed as dist
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
-from . import functional as Fn, native, use_native
+from . import backward_follows, functional as Fn, native, use_native
 
 ALIGN = 128
 
@@ -50,6 +52,66 @@ def router_top2(logits: torch.Tensor):
     if use_native(logits, "router"):
         return _RouterTop2.apply(logits)
     return Fn.router_top2_ref(logits, 2)
+
+
+class _RouteTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, sigmoid, bias, groups, top_groups, two_best, renormalize, scale):
+        weights, idx = native.route_topk_fwd(logits, k, sigmoid, bias, groups, top_groups, two_best, renormalize, scale)
+        ctx.save_for_backward(logits, weights, idx)
+        ctx.how = (sigmoid, renormalize, scale)
+        ctx.mark_non_differentiable(idx)
+        return weights, idx
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, _didx):
+        return (native.route_topk_bwd(dweights.contiguous(), *ctx.saved_tensors, *ctx.how),) + (None,) * 8
+
+
+def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
+               top_groups: int | None = None, group_score: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """``(weights fp32 [T, k], idx int64 [T, k])`` for ``logits [T, E]`` (fp32, bf16 or fp16; up to 1024 experts, 32 of them
+    chosen, 32 groups): what ``moe_ffn`` takes.
+
+    ``score``         ``"softmax"`` over all experts or ``"sigmoid"`` of each
+    ``bias``          fp32 ``[E]``, finite: added to the scores for the choice, not for the weights; it has no gradient
+    ``groups``        runs of ``E / groups`` experts; the ``top_groups`` best stay (default: all), by their best key, or with
+                      ``group_score=2`` by the sum of their two best
+    ``renormalize``   divide the chosen scores by their sum
+    ``scale``         factor of the weights
+
+    Experts come best first, the lower index first where two are equal; without a bias they are compared by their logits.  The
+    choice is that of exact arithmetic: scores that are too close for fp32 are compared in fp64.  A logit of -inf (or NaN)
+    masks an expert: it comes after all others of the chosen groups, with weight 0; +inf counts as the largest number."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [tokens, experts], got {tuple(logits.shape)}")
+    if not logits.dtype.is_floating_point:
+        raise TypeError(f"logits must be floating point, got {logits.dtype}")
+    experts = logits.shape[1]
+    top_groups = groups if top_groups is None else top_groups
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"score must be softmax or sigmoid, got {score!r}")
+    if not (1 <= groups <= 32 and experts >= 1 and experts % groups == 0 and 1 <= top_groups <= groups):
+        raise ValueError(f"{experts} experts cannot form {groups} groups of which {top_groups} stay (at most 32 groups)")
+    if not 1 <= k <= min(32, experts // groups * top_groups):
+        raise ValueError(f"k = {k} must be between 1 and the {experts // groups * top_groups} experts to choose from, at most 32")
+    if experts > 1024:
+        raise ValueError(f"at most 1024 experts, got {experts}")
+    if group_score not in (1, 2) or (group_score == 2 and experts // groups < 2):
+        raise ValueError(f"group_score must be 1 or, for groups of two experts or more, 2, got {group_score}")
+    if not (math.isfinite(scale) and scale != 0):
+        raise ValueError(f"scale must be finite and not zero, got {scale}")
+    if bias is not None:
+        if bias.shape != (experts,) or bias.device != logits.device:
+            raise ValueError(f"bias must be [{experts}] on {logits.device}, got {tuple(bias.shape)} on {bias.device}")
+        bias = bias.detach().float().contiguous()
+    if not use_native(logits, "route"):
+        return Fn.route_topk_ref(logits, k, score, bias, groups, top_groups, group_score, renormalize, scale)
+    how = (k, score == "sigmoid", bias, groups, top_groups, group_score == 2, bool(renormalize), float(scale))
+    if backward_follows(logits):
+        return _RouteTopk.apply(logits.contiguous(), *how)
+    return native.route_topk_fwd(logits.contiguous(), *how)
 
 
 # ----------------------------------------------------------------------------- plan
@@ -238,11 +300,13 @@ def aux_loss_from(logits, idx, num_experts_total: int, k: int, group=None):
 
 def moe_ffn(x: torch.Tensor, weights: torch.Tensor, idx: torch.Tensor, w1, w2, w3, *,
             group=None, recompute: bool = False, budget=None) -> torch.Tensor:
-    """Dispatch ``x [T, D]`` to its top-2 experts, run them, combine with the
-    renormalised weights.  ``w1, w3: [E_local, d_ff, D]``, ``w2: [E_local, D, d_ff]``."""
+    """Dispatch ``x [T, D]`` to its experts ``idx [T, k]``, run them, combine with ``weights``.  ``w1, w3: [E_local, d_ff,
+    D]``, ``w2: [E_local, D, d_ff]``.  On one rank the kernels take up to 32 experts per token out of up to 1024."""
     tokens, k = idx.shape
     ep = 1 if group is None else dist.get_world_size(group)
     if use_native(x, "moe") and ep == 1:
+        if not 1 <= k <= 32:
+            raise ValueError(f"between 1 and 32 experts per token, got {k}")
         from .moe_fused import moe_ffn_fused
         return moe_ffn_fused(x, weights, idx, w1, w2, w3, recompute=recompute, budget=budget)
     plan = build_plan(idx, w1.shape[0] * ep, group)

@@ -55,10 +55,11 @@ def _experts_forward(x, weights, idx, w1, w2, w3, recompute, budget, wants_grad,
     """Plan, gather, gate/up, down projection and combine.  Returns ``(out, recompute, ledger, saved)``; the last of
     ``saved`` are the experts' slot counts."""
     tokens, dim = x.shape
-    experts = w1.shape[0]
-    cap = capacity_rows(tokens * 2, experts)
+    experts, k = w1.shape[0], idx.shape[1]
+    per_token = {} if k == 2 else {"k": k}
+    cap = capacity_rows(tokens * k, experts)
     slot_row, row_slot, offs, tile_expert, meta, counts = native.moe_plan(idx, experts, cap)
-    x_perm = native.moe_gather(x, row_slot, meta, cap)
+    x_perm = native.moe_gather(x, row_slot, meta, cap, **per_token)
     tiles = meta[0:1]
     # what this call keeps for its backward pass: the permuted input and the expert outputs always, the
     # gate/up pre-activations while the stage's activation budget has room for them
@@ -71,7 +72,7 @@ def _experts_forward(x, weights, idx, w1, w2, w3, recompute, budget, wants_grad,
     keep = wants_grad and not recompute
     h, gate, up = native.gemm_swiglu(x_perm, w1, w3, tile_expert, tiles, save_gate_up=keep, align256=True)
     y_perm = native.gemm_nt(h, w2, tile_expert=tile_expert, num_m_tiles=tiles, num_experts=experts, align256=True)
-    out = native.moe_combine(y_perm, slot_row, weights, tokens, residual=residual)
+    out = native.moe_combine(y_perm, slot_row, weights, tokens, residual=residual, **per_token)
     saved = [x_perm, y_perm, weights, offs, tile_expert, meta, slot_row, row_slot]
     if keep:
         saved += [gate, up]
@@ -81,15 +82,17 @@ def _experts_forward(x, weights, idx, w1, w2, w3, recompute, budget, wants_grad,
 def _experts_backward(dout, saved, counts, w1, w2, w3, recompute):
     """Returns ``(dx_perm, dweights, dw1, dw2, dw3)``."""
     x_perm, y_perm, weights, offs, tile_expert, meta, slot_row, row_slot = saved[:8]
-    tokens, cap, experts = weights.shape[0], x_perm.shape[0], w1.shape[0]
+    tokens, k = weights.shape
+    cap, experts = x_perm.shape[0], w1.shape[0]
+    per_token = {} if k == 2 else {"k": k}
     tiles = meta[0:1]
     if recompute:
         _, gate, up = native.gemm_swiglu(x_perm, w1, w3, tile_expert, tiles, save_gate_up=True, align256=True)
     else:
         gate, up = saved[8:10]
-    dweights = torch.empty(tokens, 2, dtype=torch.float32, device=dout.device)   # every slot has its row
+    dweights = torch.empty(tokens, k, dtype=torch.float32, device=dout.device)   # every slot has its row
     dy_perm = native.moe_gather(dout, row_slot, meta, cap, scale=weights.view(-1), y_perm=y_perm,
-                                dweights=dweights.view(-1))
+                                dweights=dweights.view(-1), **per_token)
     dgu, h = native.gemm_nn_swiglu_bwd(dy_perm, w2, gate, up, tile_expert=tile_expert, num_m_tiles=tiles,
                                        num_experts=experts, align256=True, live_rows=meta[1:2])
     del gate, up
@@ -118,7 +121,8 @@ class _MoEFused(torch.autograd.Function):
     def backward(ctx, dout):
         *saved, counts = ctx.saved_tensors
         dx_perm, dweights, dw1, dw2, dw3 = _experts_backward(dout.contiguous(), saved, counts, *ctx.params, ctx.recompute)
-        dx = native.moe_combine(dx_perm, saved[6], None, dweights.shape[0])
+        tokens, k = dweights.shape
+        dx = native.moe_combine(dx_perm, saved[6], None, tokens, **({} if k == 2 else {"k": k}))
         if ctx.ledger is not None:
             ctx.budget.leave(*ctx.ledger)
         return dx, dweights, None, dw1, dw2, dw3, None, None, None

@@ -8,6 +8,7 @@ library's kernels (the benchmark reports it).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -30,7 +31,8 @@ _FAMILIES = {
     "gemm": "b2_gemm_nt", "rmsnorm": "b2_rmsnorm_fwd", "router": "b2_router_top2_fwd",
     "lmhead_ce": "b2_cross_entropy2", "adamw": "b2_adamw", "embedding": "b2_embedding_fwd",
     "rope": "b2_rope", "moe": "b2_moe_plan", "attention": "b2_attention_fwd_ex", "comm": "b2_comm_allreduce",
-    "swiglu": "b2_swiglu_bwd", "zero": "b2_zero",
+    "swiglu": "b2_swiglu_bwd", "zero": "b2_zero", "route": "b2_route_topk", "gated_norm": "b2_gated_norm_fwd",
+    "fp8": "b2_gemm_fp8",
 }
 
 
@@ -459,6 +461,72 @@ def rmsnorm_bwd(dy, x, weight, rstd, residual_grad=None):
     return dx.view(x.shape), dw
 
 
+def gated_norm_fwd(x, delta, delta_weight, weight, gate, kind: int, seq: int, residual_scale: float, eps: float):
+    """``x, delta [..., D]`` contiguous -> ``(summed, normed, stats)``, the latter 1 / rms of delta and of the sum; ``kind`` of
+    gate and layouts as in ``csrc/gated_norm.cu``."""
+    D = x.shape[-1]
+    rows = x.numel() // D
+    summed, normed = torch.empty_like(x), torch.empty_like(x)
+    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+    if rows:
+        with _on(x):
+            _call("b2_gated_norm_fwd", _p(x), _p(delta), _p(delta_weight), _p(weight), _p(gate), _p(summed), _p(normed),
+                  _p(stats), _p(stats[1]), _I(rows), _I(D), _I(seq), _I(_float_type(x, "x")), _I(kind),
+                  _I(int(gate is not None and gate.dtype == torch.float32)), _F(residual_scale), _F(eps), _stream())
+    return summed, normed, stats
+
+
+def gated_norm_bwd(dsummed, dnormed, x, delta, delta_weight, weight, gate, stats, kind: int, seq: int, residual_scale: float):
+    """Gradients ``(dx, ddelta, ddelta_weight, dweight, dgate)``; either incoming gradient may be ``None``."""
+    D = x.shape[-1]
+    rows = x.numel() // D
+    dx, ddelta = torch.empty_like(x), torch.empty_like(x)
+    dgate = None if gate is None else torch.empty_like(gate)
+    if not rows:
+        zero = torch.zeros(2, D, dtype=torch.float32, device=x.device)
+        return dx, ddelta, zero[0], zero[1], None if dgate is None else dgate.zero_()
+    dweights = torch.empty(2, D, dtype=torch.float32, device=x.device)
+    with _on(x):
+        size = require().b2_gated_norm_bwd_floats
+        size.restype = _L
+        partial = torch.empty(size(_I(rows), _I(D), _I(seq), _I(kind)), dtype=torch.float32, device=x.device)
+        _call("b2_gated_norm_bwd", _p(dsummed), _p(dnormed), _p(x), _p(delta), _p(delta_weight), _p(weight), _p(gate),
+              _p(stats[0]), _p(stats[1]), _p(dx), _p(ddelta), _p(dweights[0]), _p(dweights[1]), _p(dgate), _p(partial),
+              _I(rows), _I(D), _I(seq), _I(_FLOATS[x.dtype]), _I(kind),
+              _I(int(gate is not None and gate.dtype == torch.float32)), _F(residual_scale), _stream(), n=2)
+    return dx, ddelta, dweights[0], dweights[1], dgate
+
+
+# ------------------------------------------------------------------------------ 8-bit products
+def quantize_fp8(x, block_rows: int):
+    """``x [M, K]`` (rows of unit stride) -> e4m3 values, rows of a multiple of 16 bytes, and fp32 scales: per row and 128
+    columns (stored column by column), or per 128 x 128 values."""
+    M, K = x.shape
+    pitch, blocks = (K + 15) // 16 * 16, (K + 127) // 128
+    values = torch.empty(M, pitch, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((blocks, M) if block_rows == 1 else ((M + 127) // 128, blocks), dtype=torch.float32, device=x.device)
+    if M:
+        with _on(x):
+            _call("b2_quantize_fp8", _p(x), _I(_float_type(x, "x")), _p(values), _p(scales), _L(M), _I(K), _L(x.stride(0)),
+                  _L(pitch), _L(M), _I(block_rows), _stream())
+    return values[:, :K], scales.t() if block_rows == 1 else scales
+
+
+def gemm_fp8(a, a_scales, w, w_scales, nn: bool = False):
+    """``a [M, K]`` times ``w [N, K]`` transposed, or (``nn``) times ``w [K, N]``; ``w_scales`` always as ``w`` is stored."""
+    M, K = a.shape
+    N = w.shape[1] if nn else w.shape[0]
+    out = torch.empty(M, N, dtype=torch.bfloat16, device=a.device)
+    along_n, along_k = (1, 0) if nn else (0, 1)
+    if M:
+        with _on(a):
+            _call("b2_gemm_fp8", _p(a), _p(a_scales), _p(w), _p(w_scales), _p(out), _I(M), _I(N), _I(K), _L(a.stride(0)),
+                  _L(w.stride(0)), _L(a_scales.stride(0)), _L(a_scales.stride(1)), _L(w_scales.stride(along_n)),
+                  _L(w_scales.stride(along_k)), _I(int(nn)), _p(status_word(a.device)), _stream(),
+                  tag=f"{'NN ' if nn else ''}N={N} K={K}")
+    return out
+
+
 # ------------------------------------------------------------------------------ router
 def router_top2_fwd(logits):
     logits = logits.float().contiguous()
@@ -487,6 +555,44 @@ def router_fwd(x, w):
     idx = torch.empty(T, 2, dtype=torch.int64, device=x.device)
     _call("b2_router_fwd", _p(_bf16(x)), _p(_bf16(w)), _p(weights), _p(idx), _p(probs), _I(T), _I(E), _I(K), _stream())
     return weights, idx, probs
+
+
+_FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # types of the kernels that take all three
+
+
+def _float_type(t, what: str) -> int:
+    kind = _FLOATS.get(t.dtype)
+    if kind is None:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return kind
+
+
+def _on(t):
+    """Makes the device of ``t`` the current one, whose current stream the launches of this module go to."""
+    return contextlib.nullcontext() if t.get_device() == _raw_device() else torch.cuda.device(t.device)
+
+
+def route_topk_fwd(logits, k, sigmoid, bias, groups, top_groups, two_best, renormalize, scale):
+    """``logits [T, E]`` -> ``(weights fp32 [T, k], idx int64 [T, k])``; see ``csrc/route.cu``."""
+    T, E = logits.shape
+    kind = _float_type(logits, "logits")
+    weights = torch.empty(T, k, dtype=torch.float32, device=logits.device)
+    idx = torch.empty(T, k, dtype=torch.int64, device=logits.device)
+    if T:
+        with _on(logits):
+            _call("b2_route_topk", _p(logits), _p(bias), _p(weights), _p(idx), _L(T), _I(E), _I(k), _I(kind),
+                  _I(int(sigmoid)), _I(groups), _I(top_groups), _I(int(two_best)), _I(int(renormalize)), _F(scale), _stream())
+    return weights, idx
+
+
+def route_topk_bwd(dweights, logits, weights, idx, sigmoid, renormalize, scale):
+    T, E = logits.shape
+    dlogits = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
+    if T:
+        with _on(logits):
+            _call("b2_route_topk_bwd", _p(logits), _p(weights), _p(idx), _p(dweights), _p(dlogits), _L(T), _I(E),
+                  _I(idx.shape[1]), _I(_FLOATS[logits.dtype]), _I(int(sigmoid)), _I(int(renormalize)), _F(scale), _stream())
+    return dlogits
 
 
 # ------------------------------------------------------------------------------ loss
@@ -714,18 +820,28 @@ def moe_plan(idx, num_experts, capacity_rows):
     return slot_row, row_slot, offs, tile_expert, meta, counts
 
 
-def moe_gather(x, row_slot, meta, capacity_rows, scale=None, y_perm=None, dweights=None, out=None):
+def moe_gather(x, row_slot, meta, capacity_rows, scale=None, y_perm=None, dweights=None, out=None, k: int = 2):
     D = x.shape[1]
     if out is None:
         out = torch.empty(capacity_rows, D, dtype=torch.bfloat16, device=x.device)
+    if k != 2:
+        _call("b2_moe_gather_k", _p(_bf16(x)), _p(row_slot), _p(meta), _p(scale), _p(y_perm), _p(dweights), _p(out), _I(D),
+              _I(capacity_rows), _I(k * x.shape[0]), _I(k), _stream())
+        return out
     _call("b2_moe_gather", _p(_bf16(x)), _p(row_slot), _p(meta), _p(scale), _p(y_perm), _p(dweights), _p(out), _I(D),
           _I(capacity_rows), _I(2 * x.shape[0]), _stream())
     return out
 
 
-def moe_combine(y_perm, slot_row, weights, tokens, residual=None):
+def moe_combine(y_perm, slot_row, weights, tokens, residual=None, k: int = 2):
     D = y_perm.shape[1]
     out = torch.empty(tokens, D, dtype=torch.bfloat16, device=y_perm.device)
+    if k != 2:
+        if residual is not None:
+            raise ValueError("the residual sum rides in the combine of two experts per token only")
+        _call("b2_moe_combine_k", _p(_bf16(y_perm)), _p(slot_row), _p(weights), _p(out), _I(tokens), _I(D),
+              _I(y_perm.shape[0]), _I(k), _stream())
+        return out
     _call("b2_moe_combine", _p(_bf16(y_perm)), _p(slot_row), _p(weights), _p(residual), _p(out), _I(tokens), _I(D),
           _I(y_perm.shape[0]), _stream())
     return out

@@ -10,13 +10,18 @@
 // The backward pass forms s again from x and delta, which the caller keeps anyway, instead of reading the rounded sum.
 //
 // Both directions are bound by memory traffic: 4 tensors forward, 6 backward, a gate for each element one and two more.
-// A row is in the registers of W warps; 8 columns of a lane are one access.  All arithmetic is fp32.
+// W warps work on a row, 8 columns of a lane are one access, all arithmetic is fp32.  There are two forms of each kernel.  The
+// one for many rows brings blocks of rows into a ring in shared memory by bulk copies: a row goes through two
+// sums over its columns one after the other, forward and backward, and without rows that arrive meanwhile an SM waits most of the
+// time.  The other reads straight from global memory: for few rows, where there is nothing to read ahead, and for rows that bulk
+// copies do not take (widths that are no multiple of 8, addresses off a 16-byte boundary).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "chain.cuh"
+#include "ptx.cuh"
 
 namespace b2 {
 
@@ -40,8 +45,9 @@ struct GatedNormParams {
   void* dx;
   void* ddelta;
   void* dgate;               // [rows] or [rows, D] (GATE_TOKEN, GATE_FULL)
-  float* partial;            // [2][CTAs][D] column sums, then for GATE_SEQUENCE [workers + sequences][D]
-  int rows, D, seq, gate_kind, gate_f32, aligned;
+  float* partial;            // [2][CTAs][D] column sums, then for GATE_SEQUENCE [CTAs + sequences][rows at a time][D]
+  int* status;               // device word, non-zero: a wait ran out
+  int rows, D, seq, gate_kind, gate_f32, aligned, stages;
   float residual_scale, eps;
 };
 
@@ -201,32 +207,59 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_fwd_kernel(const G
   }
 }
 
-// A worker is W warps that share a row.  Each has a run of rows, at least one: those beyond the number of rows have none.
-__host__ __device__ __forceinline__ long long gn_workers(long long ctas, int per_cta, long long rows) {
-  return ctas * per_cta < rows ? ctas * per_cta : rows;
+// The backward kernels give each CTA a run of rows, at least one, which its slots (of W warps) take in turn.
+__host__ __device__ __forceinline__ long long gn_first_row(long long cta, long long rows, long long ctas) {
+  return cta * rows / ctas;
 }
-__host__ __device__ __forceinline__ long long gn_first_row(long long worker, long long rows, long long workers) {
-  return worker * rows / workers;
+__host__ __device__ __forceinline__ long long gn_cta_of(long long row, long long rows, long long ctas) {
+  return ((row + 1) * ctas - 1) / rows;
 }
-__host__ __device__ __forceinline__ long long gn_worker_of(long long row, long long rows, long long workers) {
-  return ((row + 1) * workers - 1) / rows;
+
+// One row of column sums per CTA: its slots' sums are added in their order through ``columns`` (a row for each of two sums).
+template <int R, int W, int THREADS>
+__device__ __forceinline__ void gn_store_sums(const GatedNormParams& p, float (&dw)[GN_VECS][8], float (&dwd)[GN_VECS][8],
+                                              float* columns, int slot, int in_row, int lane) {
+  constexpr int V = GN_VECS, WIDTH = W * 32 * 8 * V;
+  if (R > 1) {
+    for (int k = 0; k < R; ++k) {
+      asm volatile("bar.sync 15, %0;" ::"r"(THREADS) : "memory");
+      if (slot != k) continue;
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        const int col = ((c * W + in_row) * 32 + lane) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          columns[col + i] = dw[c][i] += k ? columns[col + i] : 0.f;
+          columns[WIDTH + col + i] = dwd[c][i] += k ? columns[WIDTH + col + i] : 0.f;
+        }
+      }
+    }
+    if (slot != R - 1) return;
+  }
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const int col = ((c * W + in_row) * 32 + lane) * 8;
+    Eight<float> f;
+    f.set(dw[c]);
+    f.store(p.partial + static_cast<long long>(blockIdx.x) * p.D, col, p.D, p.aligned);
+    f.set(dwd[c]);
+    f.store(p.partial + (static_cast<long long>(gridDim.x) + blockIdx.x) * p.D, col, p.D, p.aligned);
+  }
 }
 
 // Column sums stay in registers while a worker goes through its rows: dw and, where a gate of its own has no column sum, dw_d.
 // With a gate that rows share the sum a = sum of dS nhat gives both its gradient, w_d a, and dw_d, g a; for a gate per sequence a
-// is stored wherever the sequence changes, in place ``sequence + worker``, which no other pair has.
+// is stored wherever the sequence changes, in place ``sequence + CTA`` and slot, which no other has.
 template <typename T, int W, int GATE>       // GATE: 0 no column sums, 1 a gate per channel, 2 a gate per sequence
 __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const GatedNormParams p) {
   chain_begin();
   constexpr int R = gn_rows<W>(), V = GN_VECS;
   __shared__ float scratch[2][R][W];
-  __shared__ float columns[R > 1 ? 2 : 1][R > 1 ? W * 32 * 8 * V : 1];
+  __shared__ float columns[R > 1 ? 2 * W * 32 * 8 * V : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = warp / W, in_row = warp % W;
   const int D = p.D;
   const float inv = 1.f / D;
-  const long long workers = gn_workers(gridDim.x, R, p.rows), worker = static_cast<long long>(blockIdx.x) * R + slot;
-  const long long begin = worker < workers ? gn_first_row(worker, p.rows, workers) : 0;
-  const long long end = worker < workers ? gn_first_row(worker + 1, p.rows, workers) : 0;
+  const long long begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
   float dw[V][8], dwd[V][8], a[GATE == 2 ? V : 1][8];
 #pragma unroll
   for (int c = 0; c < V; ++c) {
@@ -237,8 +270,7 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const G
     }
   }
   float* const sequences = p.partial + 2LL * gridDim.x * D;
-  long long left = GATE == 2 && begin < end ? p.seq - begin % p.seq : 0;      // rows up to the end of the sequence
-  for (long long row = begin; row < end; ++row) {
+  for (long long row = begin + slot; row < end; row += R) {
     const long long at = row * D;
     Eight<T> xr[V], dr[V], sr[V], yr[V];
 #pragma unroll
@@ -342,68 +374,486 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const G
       e.set(out);
       e.store(static_cast<T*>(p.ddelta) + at, col, D, p.aligned);
     }
-    if (GATE == 2 && (--left == 0 || row + 1 == end)) {
-      left = p.seq;
-      float* dst = sequences + (row / p.seq + worker) * D;
+    if (GATE == 2 && (row + R >= end || row / p.seq != (row + R) / p.seq)) {
+      float* dst = sequences + ((row / p.seq + blockIdx.x) * R + slot) * D;
 #pragma unroll
       for (int c = 0; c < V; ++c) {
         const int col = ((c * W + in_row) * 32 + lane) * 8;
         Eight<float> f;
         f.set(a[c]);
-        f.store(dst, col, D, D % 4 == 0 && p.aligned);
+        f.store(dst, col, D, p.aligned);
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[c][i] = 0.f;
       }
     }
   }
-  // one row of sums per CTA: its rows' sums are added in the order of the slots
-  if (R > 1) {
-    for (int k = 0; k < R; ++k) {
-      __syncthreads();
-      if (slot != k) continue;
+  gn_store_sums<R, W, gn_threads<W>()>(p, dw, dwd, columns, slot, in_row, lane);
+}
+
+// ------------------------------------------------------------------ many rows: a ring of bulk copies
+constexpr int GN_RING = 4;
+
+struct GnBars {
+  uint64_t full[GN_RING], empty[GN_RING];
+};
+
+// The ring of a CTA: blocks of R consecutive rows of TENSORS tensors (null ones are left out), ``first``, ``first + step``, ... below
+// ``end``.  Thread 0 issues the copies beside its own work (a warp for them would take registers of a third of the others): the first
+// ones at the start, the next into a stage once all warps have let go of it.  A row of tensor i has ``row_bytes[i]`` bytes; its place in
+// a stage is that of the first TENSORS - 1 of ``row_bytes[0]``.
+template <int R, int TENSORS>
+struct GnRing {
+  const uint8_t* src[TENSORS];
+  uint32_t row_bytes[TENSORS];
+  uint8_t* smem;
+  uint32_t stage_bytes;
+  int stages;
+  long long first, step, end;
+
+  __device__ __forceinline__ void issue(GnBars& bars, int s, long long row) const {
+    const uint32_t rows = static_cast<uint32_t>(end - row < R ? end - row : R);
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int i = 0; i < TENSORS; ++i) bytes += src[i] ? rows * row_bytes[i] : 0;
+    mbar_expect_tx(&bars.full[s], bytes);
+#pragma unroll
+    for (int i = 0; i < TENSORS; ++i)
+      if (src[i])
+        bulk_load(smem + s * stage_bytes + i * R * row_bytes[0], src[i] + row * row_bytes[i], &bars.full[s], rows * row_bytes[i]);
+  }
+  __device__ __forceinline__ void start(GnBars& bars) const {
+    for (int s = 0; s < stages && first + s * step < end; ++s) issue(bars, s, first + s * step);
+  }
+  // The stage of block ``turn`` gets block ``turn + stages``.
+  __device__ __forceinline__ void refill(GnBars& bars, int turn, int* status) const {
+    const long long row = first + (turn + static_cast<long long>(stages)) * step;
+    if (turn < 0 || row >= end) return;
+    if (mbar_wait(&bars.empty[turn % stages], (turn / stages) & 1)) issue(bars, turn % stages, row);
+    else atomicExch(status, 6);                   // the warps that wait for this block give up in turn
+  }
+  // A CTA that gave up waits (with a limit) for what may be in flight before its shared memory goes to another one.
+  __device__ __forceinline__ void drain(GnBars& bars, int turns) const {
+    for (int i = turns < stages ? 0 : turns - stages; i < turns; ++i) mbar_wait(&bars.full[i % stages], (i / stages) & 1);
+  }
+};
+
+template <int WARPS>
+__device__ __forceinline__ void gn_init(GnBars& bars) {
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < GN_RING; ++s) {
+      mbar_init(&bars.full[s], 1);
+      mbar_init(&bars.empty[s], WARPS);
+    }
+    mbar_fence_init();
+  }
+  __syncthreads();
+}
+
+// Waits for a stage.  A warp whose wait ran out reports and goes on without waiting: the warps of a row meet at barriers.
+__device__ __forceinline__ void gn_arrived(bool& here, uint64_t& bar, uint32_t phase, int* status, int lane) {
+  if (!here) return;
+  here = mbar_wait(&bar, phase);
+  if (!here && lane == 0) atomicExch(status, 6);
+}
+
+template <typename T>
+__device__ __forceinline__ void ring_load(const uint8_t* row, int col, float (&f)[8]) {
+  Eight<T> e;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+    reinterpret_cast<uint4*>(e.v)[i] = reinterpret_cast<const uint4*>(row + col * sizeof(T))[i];
+  e.get(f);
+}
+
+// g w_d of a lane's columns (w_d where the gate is no column vector); zeros behind column D
+template <typename T, int W, int G>
+__device__ __forceinline__ void load_gwd(const GatedNormParams& p, long long row, int in_row, int lane, float (&gwd)[GN_VECS][8]) {
+#pragma unroll
+  for (int c = 0; c < GN_VECS; ++c) {
+    const int col = ((c * W + in_row) * 32 + lane) * 8;
+    load_f32x8(p.delta_weight, col, p.D, true, gwd[c]);
+    if (G == GATE_CHANNEL || G == GATE_SEQUENCE) {
+      float g[8];
+      load_gate<T>(p, row, col, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) gwd[c][i] *= g[i];
+    }
+  }
+}
+
+template <int W> constexpr int gn_ctas_per_sm() { return W == 16 ? 1 : 2; }
+
+// One barrier per row: the sum over delta of the next row is formed before the sum over s of the present one, and both cross the
+// warps together.  A CTA has a run of rows, so that a gate per sequence is loaded once per sequence and CTA.
+template <typename T, int W, int G>
+__global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_norm_fwd_ring_kernel(const GatedNormParams p) {
+  chain_begin();
+  constexpr int R = gn_rows<W>(), V = GN_VECS, WARPS = gn_threads<W>() / 32;
+  extern __shared__ __align__(128) uint8_t gn_smem[];
+  __shared__ GnBars bars;
+  __shared__ float2 scratch[2][R][W];
+  gn_init<WARPS>(bars);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D;
+  const uint32_t row_bytes = D * sizeof(T), gate_bytes = p.gate_f32 ? D * 4 : row_bytes;
+  const uint32_t stage_bytes = R * (2 * row_bytes + (G == GATE_FULL ? gate_bytes : 0));
+  const long long begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
+  const GnRing<R, 3> ring = {{static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.delta),
+                              G == GATE_FULL ? static_cast<const uint8_t*>(p.gate) : nullptr},
+                             {row_bytes, row_bytes, gate_bytes}, gn_smem, stage_bytes, p.stages, begin, R, end};
+  if (threadIdx.x == 0) ring.start(bars);
+  const int slot = warp / W, in_row = warp % W;
+  const float inv = 1.f / D;
+  float gwd[V][8], w[V][8];
+  if (G != GATE_SEQUENCE) load_gwd<T, W, G>(p, 0, in_row, lane, gwd);
+#pragma unroll
+  for (int c = 0; c < V; ++c) load_f32x8(p.weight, ((c * W + in_row) * 32 + lane) * 8, D, true, w[c]);
+  bool here = true;
+  // sum of squares of delta's columns of this lane in a stage that has arrived
+  auto squares = [&](int stage, long long row) {
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const int col = ((c * W + in_row) * 32 + lane) * 8;
+      if (row >= end || col >= D) continue;
+      float d[8];
+      ring_load<T>(gn_smem + stage * stage_bytes + (R + slot) * row_bytes, col, d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += d[i] * d[i];
+    }
+    return sum;
+  };
+  // sums of both over the warps of a row
+  auto row_sums = [&](float a, float b, int half) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if (W == 1) return make_float2(a, b);
+    if (lane == 0) scratch[half][slot][in_row] = make_float2(a, b);
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(W * 32) : "memory");
+    float2 total = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float2 v = scratch[half][slot][i];
+      total.x += v.x;
+      total.y += v.y;
+    }
+    return total;
+  };
+  int stage = 0, turn = 0, half = 0;
+  uint32_t phase = 0;
+  int sequence = -1;
+  gn_arrived(here, bars.full[0], 0, p.status, lane);
+  float rd = rsqrtf(row_sums(squares(0, begin + slot), 0.f, 1).x * inv + p.eps);
+  for (long long block = begin; block < end; block += R, ++turn, half ^= 1) {
+    const long long row = block + slot;
+    const bool live = row < end;
+    if (G == GATE_SEQUENCE && live && static_cast<int>(row) / p.seq != sequence) {
+      sequence = static_cast<int>(row) / p.seq;
+      load_gwd<T, W, G>(p, row, in_row, lane, gwd);
+    }
+    const float token = G == GATE_TOKEN && live
+                            ? (p.gate_f32 ? static_cast<const float*>(p.gate)[row] : to_f32<T>(static_cast<const T*>(p.gate)[row]))
+                            : 1.f;
+    const uint8_t* in = gn_smem + stage * stage_bytes;
+    const float factor = G == GATE_TOKEN ? rd * token : rd;
+    float s[V][8], sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const int col = ((c * W + in_row) * 32 + lane) * 8;
+      if (!live || col >= D) continue;
+      float d[8];
+      ring_load<T>(in + slot * row_bytes, col, s[c]);
+      ring_load<T>(in + (R + slot) * row_bytes, col, d);
+      if (G == GATE_FULL) {
+        float g[8];
+        const uint8_t* gate = in + 2 * R * row_bytes + slot * gate_bytes;
+        if (p.gate_f32) ring_load<float>(gate, col, g);
+        else ring_load<T>(gate, col, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] *= g[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s[c][i] = s[c][i] * p.residual_scale + d[i] * factor * gwd[c][i];
+        sum += s[c][i] * s[c][i];
+      }
+      Eight<T> out;
+      out.set(s[c]);
+      out.store(static_cast<T*>(p.summed) + row * D, col, D, true);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.empty[stage]);
+    if (++stage == p.stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    float next = 0.f;
+    if (block + R < end) {
+      gn_arrived(here, bars.full[stage], phase, p.status, lane);
+      next = squares(stage, row + R);
+    }
+    const float2 sums = row_sums(sum, next, half);
+    if (threadIdx.x == 0) ring.refill(bars, R == 1 ? turn : turn - 1, p.status);     // with several rows at a time a block later
+    const float r = rsqrtf(sums.x * inv + p.eps);
+    if (live) {
+      if (in_row == 0 && lane == 0) {
+        p.delta_rstd[row] = rd;
+        p.rstd[row] = r;
+      }
 #pragma unroll
       for (int c = 0; c < V; ++c) {
         const int col = ((c * W + in_row) * 32 + lane) * 8;
+        if (col >= D) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[c][i] *= r * w[c][i];
+        Eight<T> out;
+        out.set(s[c]);
+        out.store(static_cast<T*>(p.normed) + row * D, col, D, true);
+      }
+    }
+    rd = rsqrtf(sums.y * inv + p.eps);
+  }
+  if (threadIdx.x == 0 && !here) ring.drain(bars, turn);
+}
+
+// A value that a second phase needs again is formed again from the row in shared memory: two CTAs per SM leave 112 registers, of
+// which the column sums and g w_d take 48.  w is read from shared memory, and so is dw_d for a gate per sequence, which is
+// touched once per sequence.
+template <typename T, int W, int G>
+__global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_norm_bwd_ring_kernel(const GatedNormParams p) {
+  chain_begin();
+  constexpr int R = gn_rows<W>(), V = GN_VECS, THREADS = gn_threads<W>(), WARPS = THREADS / 32;
+  extern __shared__ __align__(128) uint8_t gn_smem[];
+  __shared__ GnBars bars;
+  __shared__ float scratch[2][R][W];
+  gn_init<WARPS>(bars);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D;
+  const uint32_t row_bytes = D * sizeof(T), gate_bytes = p.gate_f32 ? D * 4 : row_bytes;
+  const uint32_t stage_bytes = R * (4 * row_bytes + (G == GATE_FULL ? gate_bytes : 0));
+  const long long begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
+  const GnRing<R, 5> ring = {{static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.delta),
+                              static_cast<const uint8_t*>(p.dnormed), static_cast<const uint8_t*>(p.dsummed),
+                              G == GATE_FULL ? static_cast<const uint8_t*>(p.gate) : nullptr},
+                             {row_bytes, row_bytes, row_bytes, row_bytes, gate_bytes}, gn_smem, stage_bytes, p.stages, begin, R, end};
+  if (threadIdx.x == 0) ring.start(bars);
+  const int slot = warp / W, in_row = warp % W;
+  const float inv = 1.f / D;
+  float gwd[V][8], dw[V][8], a[V][8];                // a: dw_d, or the sum of dS nhat where rows share the gate
+  if (G != GATE_SEQUENCE) load_gwd<T, W, G>(p, 0, in_row, lane, gwd);
+  // a thread's own columns of w, four at a time, then those of dw_d
+  float4* const w_smem = reinterpret_cast<float4*>(gn_smem + p.stages * stage_bytes) + threadIdx.x;      // [V * 2][THREADS]
+  float* const dwd_smem = reinterpret_cast<float*>(w_smem - threadIdx.x + V * 2 * THREADS) + threadIdx.x;      // [V * 8][THREADS]
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    float w[8];
+    load_f32x8(p.weight, ((c * W + in_row) * 32 + lane) * 8, D, true, w);
+    w_smem[2 * c * THREADS] = make_float4(w[0], w[1], w[2], w[3]);
+    w_smem[(2 * c + 1) * THREADS] = make_float4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      dw[c][i] = a[c][i] = 0.f;
+      if (G == GATE_SEQUENCE) dwd_smem[(c * 8 + i) * THREADS] = 0.f;
+    }
+  }
+  auto load_w = [&](int c, float (&w)[8]) {
+    const float4 lo = w_smem[2 * c * THREADS], hi = w_smem[(2 * c + 1) * THREADS];
+    w[0] = lo.x; w[1] = lo.y; w[2] = lo.z; w[3] = lo.w; w[4] = hi.x; w[5] = hi.y; w[6] = hi.z; w[7] = hi.w;
+  };
+  float* const sequences = p.partial + 2LL * gridDim.x * D;
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  bool here = true;
+  int sequence = -1;
+  for (long long block = begin; block < end; block += R, ++turn) {
+    const long long row = block + slot, at = row * D;
+    const bool live = row < end;
+    if (G == GATE_SEQUENCE && live && static_cast<int>(row) / p.seq != sequence) {
+      sequence = static_cast<int>(row) / p.seq;
+      load_gwd<T, W, G>(p, row, in_row, lane, gwd);
+    }
+    const float rd = live ? p.delta_rstd[row] : 0.f, r = live ? p.rstd[row] : 0.f;
+    const float token = G == GATE_TOKEN && live
+                            ? (p.gate_f32 ? static_cast<const float*>(p.gate)[row] : to_f32<T>(static_cast<const T*>(p.gate)[row]))
+                            : 1.f;
+    const uint8_t* const x_row = gn_smem + stage * stage_bytes + slot * row_bytes;
+    const uint8_t* const d_row = x_row + R * row_bytes;
+    const uint8_t* const dy_row = d_row + R * row_bytes;
+    const uint8_t* const ds_row = dy_row + R * row_bytes;
+    const uint8_t* const g_row = gn_smem + stage * stage_bytes + 4 * R * row_bytes + slot * gate_bytes;
+    gn_arrived(here, bars.full[stage], phase, p.status, lane);
+    float hat[V][8];                                   // of the sum, then dn w_d
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const int col = ((c * W + in_row) * 32 + lane) * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) hat[c][i] = 0.f;
+      if (!live || col >= D) continue;
+      float d[8], x[8];
+      ring_load<T>(x_row, col, x);
+      ring_load<T>(d_row, col, d);
+      if (G == GATE_FULL) {
+        float g[8];
+        if (p.gate_f32) ring_load<float>(g_row, col, g);
+        else ring_load<T>(g_row, col, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] *= g[i];
+      }
+      const float factor = G == GATE_TOKEN ? rd * token : rd;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) hat[c][i] = (x[i] * p.residual_scale + d[i] * factor * gwd[c][i]) * r;
+      if (p.dnormed) {
+        float dy[8], w[8];
+        ring_load<T>(dy_row, col, dy);
+        load_w(c, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          columns[0][col + i] = dw[c][i] += k ? columns[0][col + i] : 0.f;
-          columns[R > 1 ? 1 : 0][col + i] = dwd[c][i] += k ? columns[R > 1 ? 1 : 0][col + i] : 0.f;
+          const float t = dy[i] * hat[c][i];
+          dw[c][i] += t;
+          sum += t * w[i];
         }
       }
     }
-    if (slot != R - 1) return;
-  }
+    const float mean = gn_row_sum<W>(sum, scratch[0], slot, in_row, lane) * inv;
+    Eight<T> dr[V];
+    sum = 0.f;
 #pragma unroll
-  for (int c = 0; c < V; ++c) {
-    const int col = ((c * W + in_row) * 32 + lane) * 8;
-    Eight<float> f;
-    f.set(dw[c]);
-    f.store(p.partial + static_cast<long long>(blockIdx.x) * D, col, D, p.aligned);
-    f.set(dwd[c]);
-    f.store(p.partial + (static_cast<long long>(gridDim.x) + blockIdx.x) * D, col, D, p.aligned);
+    for (int c = 0; c < V; ++c) {
+      const int col = ((c * W + in_row) * 32 + lane) * 8;
+      if (!live || col >= D) continue;
+      float d[8], ds[8], out[8];
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+        reinterpret_cast<uint4*>(dr[c].v)[i] = reinterpret_cast<const uint4*>(d_row + col * sizeof(T))[i];
+      dr[c].get(d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ds[i] = 0.f;
+      if (p.dsummed) ring_load<T>(ds_row, col, ds);
+      if (p.dnormed) {
+        float dy[8], w[8];
+        ring_load<T>(dy_row, col, dy);
+        load_w(c, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ds[i] += r * (dy[i] * w[i] - hat[c][i] * mean);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = ds[i] * p.residual_scale;
+      Eight<T> e;
+      e.set(out);
+      e.store(static_cast<T*>(p.dx) + at, col, D, true);
+      float g[8];
+      if (G == GATE_FULL) {
+        if (p.gate_f32) ring_load<float>(g_row, col, g);
+        else ring_load<T>(g_row, col, g);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float nhat = d[i] * rd, part = ds[i] * nhat;
+        if (G == GATE_FULL) {
+          out[i] = part * gwd[c][i];                               // dS n
+          a[c][i] += part * g[i];
+          hat[c][i] = ds[i] * gwd[c][i] * g[i];
+        } else {
+          a[c][i] += G == GATE_TOKEN ? part * token : part;
+          hat[c][i] = ds[i] * gwd[c][i];                           // the token's gate follows with the mean
+        }
+        sum += hat[c][i] * nhat;
+      }
+      if (G == GATE_FULL) {
+        if (p.gate_f32) {
+          Eight<float> f;
+          f.set(out);
+          f.store(static_cast<float*>(p.dgate) + at, col, D, true);
+        } else {
+          e.set(out);
+          e.store(static_cast<T*>(p.dgate) + at, col, D, true);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.empty[stage]);
+    if (++stage == p.stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    const float total = gn_row_sum<W>(sum, scratch[1], slot, in_row, lane);
+    if (threadIdx.x == 0) ring.refill(bars, R == 1 ? turn : turn - 1, p.status);
+    if (!live) continue;
+    if (G == GATE_TOKEN && in_row == 0 && lane == 0) {
+      if (p.gate_f32) static_cast<float*>(p.dgate)[row] = total;
+      else static_cast<T*>(p.dgate)[row] = from_f32<T>(total);
+    }
+    const float factor = G == GATE_TOKEN ? rd * token : rd, mean_d = total * inv * rd;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const int col = ((c * W + in_row) * 32 + lane) * 8;
+      if (col >= D) continue;
+      float d[8], out[8];
+      dr[c].get(d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = factor * (hat[c][i] - d[i] * mean_d);
+      Eight<T> e;
+      e.set(out);
+      e.store(static_cast<T*>(p.ddelta) + at, col, D, true);
+    }
+    if (G == GATE_SEQUENCE && (row + R >= end || static_cast<int>(row + R) / p.seq != sequence)) {
+      float* dst = sequences + (static_cast<long long>(sequence + blockIdx.x) * R + slot) * D;
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        const int col = ((c * W + in_row) * 32 + lane) * 8;
+        if (col >= D) continue;
+        float g[8];
+        load_gate<T>(p, row, col, g);
+        Eight<float> f;
+        f.set(a[c]);
+        f.store(dst, col, D, true);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dwd_smem[(c * 8 + i) * THREADS] += a[c][i] * g[i];
+          a[c][i] = 0.f;
+        }
+      }
+    }
   }
+  if (G == GATE_SEQUENCE) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[c][i] = dwd_smem[(c * 8 + i) * THREADS];
+    }
+  }
+  if (threadIdx.x == 0 && !here) ring.drain(bars, turn);
+  // the ring's shared memory serves the sums: every copy has landed and been read
+  gn_store_sums<R, W, THREADS>(p, dw, a, reinterpret_cast<float*>(gn_smem), slot, in_row, lane);
 }
 
 // Column sums of the partial rows: 32 columns per CTA, 16 partial rows at a time.  blockIdx.y: 0 dw; 1 dw_d, and the gradient of a
 // gate per channel; 2 + i the gradient of sequence i's gate.
-__global__ void __launch_bounds__(512) gated_norm_sums_kernel(const GatedNormParams p, int ctas, long long workers, int gate_bf16,
+__global__ void __launch_bounds__(512) gated_norm_sums_kernel(const GatedNormParams p, int ctas, int per_cta, int gate_bf16,
                                                               float* __restrict__ dw, float* __restrict__ dwd,
                                                               void* __restrict__ dgate) {
   chain_begin();
   __shared__ float parts[16][33];
   const int D = p.D, col = blockIdx.x * 32 + threadIdx.x;
   for (long long what = blockIdx.y; what < 2 + (p.gate_kind == GATE_SEQUENCE ? p.rows / p.seq : 0); what += gridDim.y) {
-    const float* src = p.partial + what * ctas * D;
-    long long first = 0, last = ctas;
-    if (what >= 2) {
-      const long long i = what - 2;
-      src = p.partial + (2LL * ctas + i) * D;
-      first = gn_worker_of(i * p.seq, p.rows, workers);
-      last = gn_worker_of((i + 1) * p.seq - 1, p.rows, workers) + 1;
-    }
     float sum = 0.f;
-    if (col < D)
-      for (long long r = first + threadIdx.y; r < last; r += 16) sum += src[r * D + col];
+    if (what < 2) {
+      const float* src = p.partial + what * ctas * D + col;
+      if (col < D)
+        for (int r = threadIdx.y; r < ctas; r += 16) sum += src[static_cast<long long>(r) * D];
+    } else if (col < D) {
+      const long long i = what - 2, low = i * p.seq, high = low + p.seq;
+      const long long first = gn_cta_of(low, p.rows, ctas), last = gn_cta_of(high - 1, p.rows, ctas) + 1;
+      const float* src = p.partial + (2LL * ctas + i * per_cta) * D + col;
+      for (long long r = first * per_cta + threadIdx.y; r < last * per_cta; r += 16) {
+        // a slot that had none of the sequence's rows in this CTA has stored nothing
+        const long long cta = r / per_cta, begin = gn_first_row(cta, p.rows, ctas), end = gn_first_row(cta + 1, p.rows, ctas);
+        const long long from = low > begin ? low : begin, rows = (high < end ? high : end) - from;
+        if ((r + per_cta - (from - begin) % per_cta) % per_cta < rows) sum += src[r * D];
+      }
+    }
     __syncthreads();
     parts[threadIdx.y][threadIdx.x] = sum;
     __syncthreads();
@@ -446,39 +896,95 @@ static int gn_sms() {
 
 static int gn_width(int D) { return D <= 512 ? 1 : D <= 1024 ? 2 : D <= 2048 ? 4 : D <= 4096 ? 8 : 16; }
 
-// CTAs of the backward kernel: two per SM (their registers allow no more), at least two rows for each worker.
+static int gn_rows_at_once(int D) { const int W = gn_width(D); return W == 16 ? 1 : 8 / W; }
+
+// CTAs of the backward kernels: two per SM, at least two blocks of rows each, so that the partial sums stay small beside the rows.
 static int gn_bwd_ctas(int rows, int D) {
-  const int W = gn_width(D), per_cta = W == 16 ? 1 : 8 / W;
-  const long long most = gn_sms() * (W == 16 ? 1LL : 2LL), wanted = (rows + 2LL * per_cta - 1) / (2LL * per_cta);
+  const int W = gn_width(D), R = gn_rows_at_once(D);
+  const long long most = gn_sms() * (W == 16 ? 1LL : 2LL), wanted = (rows + 2LL * R - 1) / (2LL * R);
   return static_cast<int>(wanted < most ? wanted : most);
 }
 
+// Bytes of one stage of the ring, and how many stages fit beside the ``extra`` bytes: of 227 KiB per SM, less 1 KiB a CTA.
+static uint32_t gn_stage_bytes(const GatedNormParams& p, int type, bool backward) {
+  const uint32_t row = p.D * (type == 0 ? 4 : 2);
+  return gn_rows_at_once(p.D) * ((backward ? 4 : 2) * row + (p.gate_kind == GATE_FULL ? (p.gate_f32 ? p.D * 4 : row) : 0));
+}
+static uint32_t gn_extra_bytes(const GatedNormParams& p, bool backward) {
+  // backward: w, and dw_d of a gate per sequence
+  return backward ? (gn_width(p.D) == 16 ? 512 : 256) * GN_VECS * 8 * 4 * (p.gate_kind == GATE_SEQUENCE ? 2 : 1) : 0;
+}
+static int gn_stages(const GatedNormParams& p, int type, bool backward) {
+  const uint32_t per_cta = (gn_width(p.D) == 16 ? 226 : 113) * 1024u - 600u - gn_extra_bytes(p, backward);
+  const uint32_t n = per_cta / gn_stage_bytes(p, type, backward);
+  return static_cast<int>(n < GN_RING ? n : GN_RING);
+}
+
+template <typename... Args>
+static cudaError_t gn_launch_ring(void (*kernel)(Args...), int ctas, int threads, uint32_t smem, cudaStream_t s, const GatedNormParams& p) {
+  // once per kernel and process; the attribute is the largest that any width asks for
+  static thread_local void* last = nullptr;
+  if (last != reinterpret_cast<void*>(kernel)) {
+    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024 - 600);
+    if (r != cudaSuccess) return r;
+    last = reinterpret_cast<void*>(kernel);
+  }
+  return launch_next(kernel, ctas, threads, smem, s, p);
+}
+
+// Which form.  A ring of two stages or more, aligned rows, and more blocks of rows than a CTA would have in one go.
 template <typename T, int W>
-static cudaError_t gn_launch(const GatedNormParams& p, bool backward, int gate_bf16, float* dw, float* dwd, cudaStream_t s) {
-  constexpr int R = gn_rows<W>();
+static cudaError_t gn_launch(GatedNormParams& p, int type, bool backward, int gate_bf16, float* dw, float* dwd, cudaStream_t s) {
+  constexpr int R = gn_rows<W>(), THREADS = gn_threads<W>();
+  const long long blocks = (p.rows + R - 1LL) / R, resident = gn_sms() * static_cast<long long>(gn_ctas_per_sm<W>());
+  p.stages = gn_stages(p, type, backward);
+  const bool ring = p.aligned && p.stages >= 2 && blocks >= 2 * resident;
+  const uint32_t smem = p.stages * gn_stage_bytes(p, type, backward) + gn_extra_bytes(p, backward);
   if (!backward) {
-    const long long blocks = (p.rows + R - 1) / R, most = gn_sms() * (W == 16 ? 4LL : 8LL);
-    return launch_next(gated_norm_fwd_kernel<T, W>, static_cast<unsigned>(blocks < most ? blocks : most), gn_threads<W>(), 0, s, p);
+    if (ring) {
+      const int ctas = static_cast<int>(resident);
+      switch (p.gate_kind) {
+        case GATE_NONE:                // as a gate per channel of ones
+        case GATE_CHANNEL: return gn_launch_ring(gated_norm_fwd_ring_kernel<T, W, GATE_CHANNEL>, ctas, THREADS, smem, s, p);
+        case GATE_SEQUENCE: return gn_launch_ring(gated_norm_fwd_ring_kernel<T, W, GATE_SEQUENCE>, ctas, THREADS, smem, s, p);
+        case GATE_TOKEN: return gn_launch_ring(gated_norm_fwd_ring_kernel<T, W, GATE_TOKEN>, ctas, THREADS, smem, s, p);
+        default: return gn_launch_ring(gated_norm_fwd_ring_kernel<T, W, GATE_FULL>, ctas, THREADS, smem, s, p);
+      }
+    }
+    const long long most = gn_sms() * (W == 16 ? 4LL : 8LL);
+    return launch_next(gated_norm_fwd_kernel<T, W>, static_cast<unsigned>(blocks < most ? blocks : most), THREADS, 0, s, p);
   }
   const int ctas = gn_bwd_ctas(p.rows, p.D);
   cudaError_t r;
-  if (p.gate_kind == GATE_CHANNEL) r = launch_next(gated_norm_bwd_kernel<T, W, 1>, ctas, gn_threads<W>(), 0, s, p);
-  else if (p.gate_kind == GATE_SEQUENCE) r = launch_next(gated_norm_bwd_kernel<T, W, 2>, ctas, gn_threads<W>(), 0, s, p);
-  else r = launch_next(gated_norm_bwd_kernel<T, W, 0>, ctas, gn_threads<W>(), 0, s, p);
+  if (ring) {
+    switch (p.gate_kind) {
+      case GATE_NONE:
+      case GATE_CHANNEL: r = gn_launch_ring(gated_norm_bwd_ring_kernel<T, W, GATE_CHANNEL>, ctas, THREADS, smem, s, p); break;
+      case GATE_SEQUENCE: r = gn_launch_ring(gated_norm_bwd_ring_kernel<T, W, GATE_SEQUENCE>, ctas, THREADS, smem, s, p); break;
+      case GATE_TOKEN: r = gn_launch_ring(gated_norm_bwd_ring_kernel<T, W, GATE_TOKEN>, ctas, THREADS, smem, s, p); break;
+      default: r = gn_launch_ring(gated_norm_bwd_ring_kernel<T, W, GATE_FULL>, ctas, THREADS, smem, s, p);
+    }
+  } else if (p.gate_kind == GATE_CHANNEL) {
+    r = launch_next(gated_norm_bwd_kernel<T, W, 1>, ctas, THREADS, 0, s, p);
+  } else if (p.gate_kind == GATE_SEQUENCE) {
+    r = launch_next(gated_norm_bwd_kernel<T, W, 2>, ctas, THREADS, 0, s, p);
+  } else {
+    r = launch_next(gated_norm_bwd_kernel<T, W, 0>, ctas, THREADS, 0, s, p);
+  }
   if (r != cudaSuccess) return r;
   const long long sums = 2 + (p.gate_kind == GATE_SEQUENCE ? p.rows / p.seq : 0);
   return launch_next(gated_norm_sums_kernel, dim3((p.D + 31) / 32, static_cast<unsigned>(sums < 32768 ? sums : 32768)),
-                     dim3(32, 16), 0, s, p, ctas, gn_workers(ctas, R, p.rows), gate_bf16, dw, dwd, p.dgate);
+                     dim3(32, 16), 0, s, p, ctas, R, gate_bf16, dw, dwd, p.dgate);
 }
 
 template <typename T>
-static cudaError_t gn_dispatch(const GatedNormParams& p, bool backward, int gate_bf16, float* dw, float* dwd, cudaStream_t s) {
+static cudaError_t gn_dispatch(GatedNormParams& p, int type, bool backward, int gate_bf16, float* dw, float* dwd, cudaStream_t s) {
   switch (gn_width(p.D)) {
-    case 1: return gn_launch<T, 1>(p, backward, gate_bf16, dw, dwd, s);
-    case 2: return gn_launch<T, 2>(p, backward, gate_bf16, dw, dwd, s);
-    case 4: return gn_launch<T, 4>(p, backward, gate_bf16, dw, dwd, s);
-    case 8: return gn_launch<T, 8>(p, backward, gate_bf16, dw, dwd, s);
-    default: return gn_launch<T, 16>(p, backward, gate_bf16, dw, dwd, s);
+    case 1: return gn_launch<T, 1>(p, type, backward, gate_bf16, dw, dwd, s);
+    case 2: return gn_launch<T, 2>(p, type, backward, gate_bf16, dw, dwd, s);
+    case 4: return gn_launch<T, 4>(p, type, backward, gate_bf16, dw, dwd, s);
+    case 8: return gn_launch<T, 8>(p, type, backward, gate_bf16, dw, dwd, s);
+    default: return gn_launch<T, 16>(p, type, backward, gate_bf16, dw, dwd, s);
   }
 }
 
@@ -495,9 +1001,9 @@ static int gated_norm(GatedNormParams& p, int type, bool backward, float* dw, fl
                         static_cast<const void*>(p.partial)})
     bits |= reinterpret_cast<uintptr_t>(t);
   p.aligned = p.D % 8 == 0 && bits % 16 == 0;
-  const cudaError_t r = type == 0   ? gn_dispatch<float>(p, backward, 0, dw, dwd, s)
-                        : type == 1 ? gn_dispatch<__nv_bfloat16>(p, backward, 1, dw, dwd, s)
-                                    : gn_dispatch<__half>(p, backward, 0, dw, dwd, s);
+  const cudaError_t r = type == 0   ? gn_dispatch<float>(p, type, backward, 0, dw, dwd, s)
+                        : type == 1 ? gn_dispatch<__nv_bfloat16>(p, type, backward, 1, dw, dwd, s)
+                                    : gn_dispatch<__half>(p, type, backward, 0, dw, dwd, s);
   if (r != cudaSuccess) cudaGetLastError();
   return r == cudaSuccess ? 0 : -1;
 }
@@ -512,31 +1018,31 @@ extern "C" {
 // ``type`` or fp32; delta_rstd, rstd fp32 [rows].
 int b2_gated_norm_fwd(const void* x, const void* delta, const float* delta_weight, const float* weight, const void* gate,
                       void* summed, void* normed, float* delta_rstd, float* rstd, int rows, int D, int seq, int type,
-                      int gate_kind, int gate_f32, float residual_scale, float eps, cudaStream_t s) {
+                      int gate_kind, int gate_f32, float residual_scale, float eps, int* status, cudaStream_t s) {
   GatedNormParams p{};
   p.x = x; p.delta = delta; p.delta_weight = delta_weight; p.weight = weight; p.gate = gate; p.summed = summed;
   p.normed = normed; p.delta_rstd = delta_rstd; p.rstd = rstd; p.rows = rows; p.D = D; p.seq = seq;
-  p.gate_kind = gate_kind; p.gate_f32 = gate_f32; p.residual_scale = residual_scale; p.eps = eps;
+  p.gate_kind = gate_kind; p.gate_f32 = gate_f32; p.residual_scale = residual_scale; p.status = status; p.eps = eps;
   return gated_norm(p, type, false, nullptr, nullptr, s);
 }
 
 // Floats of the workspace of the backward pass.
 long long b2_gated_norm_bwd_floats(int rows, int D, int seq, int gate_kind) {
   if (rows < 1 || D < 1 || D > GN_MAX_D || (gate_kind == GATE_SEQUENCE && seq < 1)) return 0;
-  const long long ctas = gn_bwd_ctas(rows, D), W = gn_width(D), R = W == 16 ? 1 : 8 / W;
-  return (2 * ctas + (gate_kind == GATE_SEQUENCE ? ctas * R + rows / seq : 0)) * D;
+  const long long ctas = gn_bwd_ctas(rows, D);
+  return (2 * ctas + (gate_kind == GATE_SEQUENCE ? (ctas + rows / seq) * gn_rows_at_once(D) : 0)) * D;
 }
 
 // Gradients; dsummed and dnormed may be null (zero).  dgate has the gate's shape and type; dw, dwd fp32 [D].
 int b2_gated_norm_bwd(const void* dsummed, const void* dnormed, const void* x, const void* delta, const float* delta_weight,
                       const float* weight, const void* gate, const float* delta_rstd, const float* rstd, void* dx, void* ddelta,
                       float* dwd, float* dw, void* dgate, float* partial, int rows, int D, int seq, int type, int gate_kind,
-                      int gate_f32, float residual_scale, cudaStream_t s) {
+                      int gate_f32, float residual_scale, int* status, cudaStream_t s) {
   GatedNormParams p{};
   p.x = x; p.delta = delta; p.delta_weight = delta_weight; p.weight = weight; p.gate = gate;
   p.delta_rstd = const_cast<float*>(delta_rstd); p.rstd = const_cast<float*>(rstd); p.dsummed = dsummed; p.dnormed = dnormed;
   p.dx = dx; p.ddelta = ddelta; p.dgate = dgate; p.partial = partial; p.rows = rows; p.D = D; p.seq = seq;
-  p.gate_kind = gate_kind; p.gate_f32 = gate_f32; p.residual_scale = residual_scale;
+  p.gate_kind = gate_kind; p.gate_f32 = gate_f32; p.residual_scale = residual_scale; p.status = status;
   return gated_norm(p, type, true, dw, dwd, s);
 }
 

@@ -472,7 +472,8 @@ def gated_norm_fwd(x, delta, delta_weight, weight, gate, kind: int, seq: int, re
         with _on(x):
             _call("b2_gated_norm_fwd", _p(x), _p(delta), _p(delta_weight), _p(weight), _p(gate), _p(summed), _p(normed),
                   _p(stats), _p(stats[1]), _I(rows), _I(D), _I(seq), _I(_float_type(x, "x")), _I(kind),
-                  _I(int(gate is not None and gate.dtype == torch.float32)), _F(residual_scale), _F(eps), _stream())
+                  _I(int(gate is not None and gate.dtype == torch.float32)), _F(residual_scale), _F(eps),
+                  _p(status_word(x.device)), _stream())
     return summed, normed, stats
 
 
@@ -493,7 +494,8 @@ def gated_norm_bwd(dsummed, dnormed, x, delta, delta_weight, weight, gate, stats
         _call("b2_gated_norm_bwd", _p(dsummed), _p(dnormed), _p(x), _p(delta), _p(delta_weight), _p(weight), _p(gate),
               _p(stats[0]), _p(stats[1]), _p(dx), _p(ddelta), _p(dweights[0]), _p(dweights[1]), _p(dgate), _p(partial),
               _I(rows), _I(D), _I(seq), _I(_FLOATS[x.dtype]), _I(kind),
-              _I(int(gate is not None and gate.dtype == torch.float32)), _F(residual_scale), _stream(), n=2)
+              _I(int(gate is not None and gate.dtype == torch.float32)), _F(residual_scale), _p(status_word(x.device)),
+              _stream(), n=2)
     return dx, ddelta, dweights[0], dweights[1], dgate
 
 

@@ -207,6 +207,17 @@ def test_gated_add_rmsnorm_types(B, S, D, kind, dtype):
         _check_norm(*_norm_case(B, S, D, kind, dtype, torch.float32))
 
 
+@pytest.mark.parametrize("kind", ["none", "channel", "sequence", "token", "full"])
+@pytest.mark.parametrize("B,S,D,dtype", [(7, 701, 512, torch.bfloat16), (3, 1001, 776, torch.float16), (2, 701, 2048, torch.bfloat16),
+                                         (601, 5, 1024, torch.bfloat16), (13, 47, 4096, torch.bfloat16), (2, 307, 5120, torch.bfloat16),
+                                         (4, 601, 264, torch.float32), (5, 80, 8192, torch.float16), (1, 617, 4096, torch.float32),
+                                         (1, 300, 8192, torch.float32), (2999, 3, 104, torch.bfloat16)])
+def test_gated_add_rmsnorm_of_many_rows(B, S, D, dtype, kind):
+    _check_norm(*_norm_case(B, S, D, kind, dtype))
+    if D in (2048, 5120):
+        _check_norm(*_norm_case(B, S, D, kind, dtype, torch.float32), use=(D == 2048, D != 2048))
+
+
 def test_gated_add_rmsnorm_uses_and_layouts():
     for use in ((True, False), (False, True)):
         _check_norm(*_norm_case(2, 30, 264, "channel", torch.bfloat16), use=use)

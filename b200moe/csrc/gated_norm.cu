@@ -60,6 +60,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return 
 template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half(v); }
 template <> __device__ __forceinline__ float from_f32(float v) { return v; }
 
+template <typename T> struct is_bf16 { static constexpr bool value = false; };
+template <> struct is_bf16<__nv_bfloat16> { static constexpr bool value = true; };
+
 // 8 columns from ``col`` on, zeros behind column D.
 template <typename T>
 struct Eight {
@@ -89,13 +92,30 @@ struct Eight {
     for (int i = 0; i < 8; ++i)
       if (col + i < D) row[col + i] = v[i];
   }
+  // two values at a time: one instruction each way for a pair of 16-bit values
   __device__ __forceinline__ void get(float (&f)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(v[i]);
+    for (int i = 0; i < 4; ++i) {
+      float2 t;
+      if constexpr (sizeof(T) == 4) t = make_float2(v[2 * i], v[2 * i + 1]);
+      else if constexpr (is_bf16<T>::value) t = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(v)[i]);
+      else t = __half22float2(reinterpret_cast<const __half2*>(v)[i]);
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
   }
   __device__ __forceinline__ void set(const float (&f)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = from_f32<T>(f[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[2 * i] = f[2 * i];
+        v[2 * i + 1] = f[2 * i + 1];
+      } else if constexpr (is_bf16<T>::value) {
+        reinterpret_cast<__nv_bfloat162*>(v)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      } else {
+        reinterpret_cast<__half2*>(v)[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      }
+    }
   }
 };
 
@@ -207,12 +227,11 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_fwd_kernel(const G
   }
 }
 
-// The backward kernels give each CTA a run of rows, at least one, which its slots (of W warps) take in turn.
-__host__ __device__ __forceinline__ long long gn_first_row(long long cta, long long rows, long long ctas) {
-  return cta * rows / ctas;
-}
-__host__ __device__ __forceinline__ long long gn_cta_of(long long row, long long rows, long long ctas) {
-  return ((row + 1) * ctas - 1) / rows;
+// A CTA has a run of rows, at least one, which its slots (of W warps) take in turn.
+__device__ __forceinline__ int gn_first_row(int cta, int rows, int ctas) { return cta * (rows / ctas) + min(cta, rows % ctas); }
+__device__ __forceinline__ int gn_cta_of(int row, int rows, int ctas) {
+  const int base = rows / ctas, longer = rows % ctas * (base + 1);          // the first ones have a row more
+  return row < longer ? row / (base + 1) : rows % ctas + (row - longer) / base;
 }
 
 // One row of column sums per CTA: its slots' sums are added in their order through ``columns`` (a row for each of two sums).
@@ -259,7 +278,7 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const G
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = warp / W, in_row = warp % W;
   const int D = p.D;
   const float inv = 1.f / D;
-  const long long begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
+  const int begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
   float dw[V][8], dwd[V][8], a[GATE == 2 ? V : 1][8];
 #pragma unroll
   for (int c = 0; c < V; ++c) {
@@ -270,8 +289,8 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const G
     }
   }
   float* const sequences = p.partial + 2LL * gridDim.x * D;
-  for (long long row = begin + slot; row < end; row += R) {
-    const long long at = row * D;
+  for (int row = begin + slot; row < end; row += R) {
+    const long long at = static_cast<long long>(row) * D;
     Eight<T> xr[V], dr[V], sr[V], yr[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) {
@@ -375,7 +394,7 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const G
       e.store(static_cast<T*>(p.ddelta) + at, col, D, p.aligned);
     }
     if (GATE == 2 && (row + R >= end || row / p.seq != (row + R) / p.seq)) {
-      float* dst = sequences + ((row / p.seq + blockIdx.x) * R + slot) * D;
+      float* dst = sequences + (static_cast<long long>(row / p.seq + blockIdx.x) * R + slot) * D;
 #pragma unroll
       for (int c = 0; c < V; ++c) {
         const int col = ((c * W + in_row) * 32 + lane) * 8;
@@ -393,59 +412,47 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const G
 // ------------------------------------------------------------------ many rows: a ring of bulk copies
 constexpr int GN_RING = 4;
 
-struct GnBars {
-  uint64_t full[GN_RING], empty[GN_RING];
-};
-
-// The ring of a CTA: blocks of R consecutive rows of TENSORS tensors (null ones are left out), ``first``, ``first + step``, ... below
-// ``end``.  Thread 0 issues the copies beside its own work (a warp for them would take registers of a third of the others): the first
-// ones at the start, the next into a stage once all warps have let go of it.  A row of tensor i has ``row_bytes[i]`` bytes; its place in
-// a stage is that of the first TENSORS - 1 of ``row_bytes[0]``.
-template <int R, int TENSORS>
+// The ring of a slot: its rows ``first``, ``first + step``, ... below ``end`` of TENSORS tensors (null ones are left out).  The first
+// lane of the slot issues the copies beside its own work (a warp for them would take registers of a third of the others): the
+// first ones at the start, the next into a stage once the slot's warps have met at the barrier behind their last read of it.
+// A row of tensor i has ``row_bytes[i]`` bytes; all but the last of a stage have those of the first.
+template <int TENSORS>
 struct GnRing {
   const uint8_t* src[TENSORS];
   uint32_t row_bytes[TENSORS];
-  uint8_t* smem;
-  uint32_t stage_bytes;
+  uint8_t* smem;             // this slot's part of stage 0
+  uint32_t stage_bytes;      // of all slots
   int stages;
-  long long first, step, end;
+  uint64_t* full;            // a barrier per stage
+  int first, step, end;
 
-  __device__ __forceinline__ void issue(GnBars& bars, int s, long long row) const {
-    const uint32_t rows = static_cast<uint32_t>(end - row < R ? end - row : R);
+  __device__ __forceinline__ void issue(int s, int row) const {
     uint32_t bytes = 0;
 #pragma unroll
-    for (int i = 0; i < TENSORS; ++i) bytes += src[i] ? rows * row_bytes[i] : 0;
-    mbar_expect_tx(&bars.full[s], bytes);
+    for (int i = 0; i < TENSORS; ++i) bytes += src[i] ? row_bytes[i] : 0;
+    mbar_expect_tx(&full[s], bytes);
 #pragma unroll
     for (int i = 0; i < TENSORS; ++i)
-      if (src[i])
-        bulk_load(smem + s * stage_bytes + i * R * row_bytes[0], src[i] + row * row_bytes[i], &bars.full[s], rows * row_bytes[i]);
+      if (src[i]) bulk_load(smem + s * stage_bytes + i * row_bytes[0], src[i] + static_cast<size_t>(row) * row_bytes[i], &full[s],
+                            row_bytes[i]);
   }
-  __device__ __forceinline__ void start(GnBars& bars) const {
-    for (int s = 0; s < stages && first + s * step < end; ++s) issue(bars, s, first + s * step);
+  __device__ __forceinline__ void start() const {
+    for (int s = 0; s < stages && first + s * step < end; ++s) issue(s, first + s * step);
   }
-  // The stage of block ``turn`` gets block ``turn + stages``.
-  __device__ __forceinline__ void refill(GnBars& bars, int turn, int* status) const {
-    const long long row = first + (turn + static_cast<long long>(stages)) * step;
-    if (turn < 0 || row >= end) return;
-    if (mbar_wait(&bars.empty[turn % stages], (turn / stages) & 1)) issue(bars, turn % stages, row);
-    else atomicExch(status, 6);                   // the warps that wait for this block give up in turn
+  // The stage of row ``row``, which has been read, gets the row that is ``stages`` further.
+  __device__ __forceinline__ void refill(int s, int row) const {
+    row += stages * step;
+    if (row < end) issue(s, row);
   }
-  // A CTA that gave up waits (with a limit) for what may be in flight before its shared memory goes to another one.
-  __device__ __forceinline__ void drain(GnBars& bars, int turns) const {
-    for (int i = turns < stages ? 0 : turns - stages; i < turns; ++i) mbar_wait(&bars.full[i % stages], (i / stages) & 1);
+  // A slot that gave up waits (with a limit) for what may be in flight before its shared memory goes to another CTA.
+  __device__ __forceinline__ void drain(int turns) const {
+    for (int i = turns < stages ? 0 : turns - stages; i < turns; ++i) mbar_wait(&full[i % stages], (i / stages) & 1);
   }
 };
 
-template <int WARPS>
-__device__ __forceinline__ void gn_init(GnBars& bars) {
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < GN_RING; ++s) {
-      mbar_init(&bars.full[s], 1);
-      mbar_init(&bars.empty[s], WARPS);
-    }
-    mbar_fence_init();
-  }
+__device__ __forceinline__ void gn_init(uint64_t* bars, int count) {
+  if (static_cast<int>(threadIdx.x) < count) mbar_init(&bars[threadIdx.x], 1);
+  mbar_fence_init();
   __syncthreads();
 }
 
@@ -488,20 +495,22 @@ template <int W> constexpr int gn_ctas_per_sm() { return W == 16 ? 1 : 2; }
 template <typename T, int W, int G>
 __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_norm_fwd_ring_kernel(const GatedNormParams p) {
   chain_begin();
-  constexpr int R = gn_rows<W>(), V = GN_VECS, WARPS = gn_threads<W>() / 32;
+  constexpr int R = gn_rows<W>(), V = GN_VECS;
   extern __shared__ __align__(128) uint8_t gn_smem[];
-  __shared__ GnBars bars;
+  __shared__ uint64_t bars[R][GN_RING];
   __shared__ float2 scratch[2][R][W];
-  gn_init<WARPS>(bars);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D;
+  gn_init(bars[0], R * GN_RING);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = warp / W, in_row = warp % W, D = p.D;
   const uint32_t row_bytes = D * sizeof(T), gate_bytes = p.gate_f32 ? D * 4 : row_bytes;
-  const uint32_t stage_bytes = R * (2 * row_bytes + (G == GATE_FULL ? gate_bytes : 0));
-  const long long begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
-  const GnRing<R, 3> ring = {{static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.delta),
-                              G == GATE_FULL ? static_cast<const uint8_t*>(p.gate) : nullptr},
-                             {row_bytes, row_bytes, gate_bytes}, gn_smem, stage_bytes, p.stages, begin, R, end};
-  if (threadIdx.x == 0) ring.start(bars);
-  const int slot = warp / W, in_row = warp % W;
+  const uint32_t slot_bytes = 2 * row_bytes + (G == GATE_FULL ? gate_bytes : 0), stage_bytes = R * slot_bytes;
+  const int begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
+  const uint8_t* const mine = gn_smem + slot * slot_bytes;
+  const GnRing<3> ring = {{static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.delta),
+                           G == GATE_FULL ? static_cast<const uint8_t*>(p.gate) : nullptr},
+                          {row_bytes, row_bytes, gate_bytes}, gn_smem + slot * slot_bytes, stage_bytes, p.stages, bars[slot],
+                          begin + slot, R, end};
+  const bool leader = in_row == 0 && lane == 0;
+  if (leader) ring.start();
   const float inv = 1.f / D;
   float gwd[V][8], w[V][8];
   if (G != GATE_SEQUENCE) load_gwd<T, W, G>(p, 0, in_row, lane, gwd);
@@ -509,14 +518,14 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
   for (int c = 0; c < V; ++c) load_f32x8(p.weight, ((c * W + in_row) * 32 + lane) * 8, D, true, w[c]);
   bool here = true;
   // sum of squares of delta's columns of this lane in a stage that has arrived
-  auto squares = [&](int stage, long long row) {
+  auto squares = [&](int stage) {
     float sum = 0.f;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const int col = ((c * W + in_row) * 32 + lane) * 8;
-      if (row >= end || col >= D) continue;
+      if (col >= D) continue;
       float d[8];
-      ring_load<T>(gn_smem + stage * stage_bytes + (R + slot) * row_bytes, col, d);
+      ring_load<T>(mine + stage * stage_bytes + row_bytes, col, d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += d[i] * d[i];
     }
@@ -543,34 +552,34 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
   };
   int stage = 0, turn = 0, half = 0;
   uint32_t phase = 0;
-  int sequence = -1;
-  gn_arrived(here, bars.full[0], 0, p.status, lane);
-  float rd = rsqrtf(row_sums(squares(0, begin + slot), 0.f, 1).x * inv + p.eps);
-  for (long long block = begin; block < end; block += R, ++turn, half ^= 1) {
-    const long long row = block + slot;
-    const bool live = row < end;
-    if (G == GATE_SEQUENCE && live && static_cast<int>(row) / p.seq != sequence) {
-      sequence = static_cast<int>(row) / p.seq;
+  int sequence_end = 0;
+  if (begin + slot >= end) return;                   // a slot's warps meet nobody else
+  gn_arrived(here, bars[slot][0], 0, p.status, lane);
+  float rd = rsqrtf(row_sums(squares(0), 0.f, 1).x * inv + p.eps);
+  for (int row = begin + slot; row < end; row += R, ++turn, half ^= 1) {
+    if (G == GATE_SEQUENCE && row >= sequence_end) {
+      sequence_end = (row / p.seq + 1) * p.seq;
       load_gwd<T, W, G>(p, row, in_row, lane, gwd);
     }
-    const float token = G == GATE_TOKEN && live
+    const float token = G == GATE_TOKEN
                             ? (p.gate_f32 ? static_cast<const float*>(p.gate)[row] : to_f32<T>(static_cast<const T*>(p.gate)[row]))
                             : 1.f;
-    const uint8_t* in = gn_smem + stage * stage_bytes;
+    const uint8_t* in = mine + stage * stage_bytes;
     const float factor = G == GATE_TOKEN ? rd * token : rd;
+    T* const summed = static_cast<T*>(p.summed) + static_cast<size_t>(row) * D;
+    T* const normed = static_cast<T*>(p.normed) + static_cast<size_t>(row) * D;
     float s[V][8], sum = 0.f;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const int col = ((c * W + in_row) * 32 + lane) * 8;
-      if (!live || col >= D) continue;
+      if (col >= D) continue;
       float d[8];
-      ring_load<T>(in + slot * row_bytes, col, s[c]);
-      ring_load<T>(in + (R + slot) * row_bytes, col, d);
+      ring_load<T>(in, col, s[c]);
+      ring_load<T>(in + row_bytes, col, d);
       if (G == GATE_FULL) {
         float g[8];
-        const uint8_t* gate = in + 2 * R * row_bytes + slot * gate_bytes;
-        if (p.gate_f32) ring_load<float>(gate, col, g);
-        else ring_load<T>(gate, col, g);
+        if (p.gate_f32) ring_load<float>(in + 2 * row_bytes, col, g);
+        else ring_load<T>(in + 2 * row_bytes, col, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[i] *= g[i];
       }
@@ -581,41 +590,38 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
       }
       Eight<T> out;
       out.set(s[c]);
-      out.store(static_cast<T*>(p.summed) + row * D, col, D, true);
+      out.store(summed, col, D, true);
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars.empty[stage]);
+    const int read = stage;
     if (++stage == p.stages) {
       stage = 0;
       phase ^= 1;
     }
     float next = 0.f;
-    if (block + R < end) {
-      gn_arrived(here, bars.full[stage], phase, p.status, lane);
-      next = squares(stage, row + R);
+    if (row + R < end) {
+      gn_arrived(here, bars[slot][stage], phase, p.status, lane);
+      next = squares(stage);
     }
     const float2 sums = row_sums(sum, next, half);
-    if (threadIdx.x == 0) ring.refill(bars, R == 1 ? turn : turn - 1, p.status);     // with several rows at a time a block later
+    if (leader) ring.refill(read, row);
     const float r = rsqrtf(sums.x * inv + p.eps);
-    if (live) {
-      if (in_row == 0 && lane == 0) {
-        p.delta_rstd[row] = rd;
-        p.rstd[row] = r;
-      }
+    if (leader) {
+      p.delta_rstd[row] = rd;
+      p.rstd[row] = r;
+    }
 #pragma unroll
-      for (int c = 0; c < V; ++c) {
-        const int col = ((c * W + in_row) * 32 + lane) * 8;
-        if (col >= D) continue;
+    for (int c = 0; c < V; ++c) {
+      const int col = ((c * W + in_row) * 32 + lane) * 8;
+      if (col >= D) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[c][i] *= r * w[c][i];
-        Eight<T> out;
-        out.set(s[c]);
-        out.store(static_cast<T*>(p.normed) + row * D, col, D, true);
-      }
+      for (int i = 0; i < 8; ++i) s[c][i] *= r * w[c][i];
+      Eight<T> out;
+      out.set(s[c]);
+      out.store(normed, col, D, true);
     }
     rd = rsqrtf(sums.y * inv + p.eps);
   }
-  if (threadIdx.x == 0 && !here) ring.drain(bars, turn);
+  if (leader && !here) ring.drain(turn);
 }
 
 // A value that a second phase needs again is formed again from the row in shared memory: two CTAs per SM leave 112 registers, of
@@ -624,21 +630,22 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
 template <typename T, int W, int G>
 __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_norm_bwd_ring_kernel(const GatedNormParams p) {
   chain_begin();
-  constexpr int R = gn_rows<W>(), V = GN_VECS, THREADS = gn_threads<W>(), WARPS = THREADS / 32;
+  constexpr int R = gn_rows<W>(), V = GN_VECS, THREADS = gn_threads<W>();
   extern __shared__ __align__(128) uint8_t gn_smem[];
-  __shared__ GnBars bars;
+  __shared__ uint64_t bars[R][GN_RING];
   __shared__ float scratch[2][R][W];
-  gn_init<WARPS>(bars);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D;
+  gn_init(bars[0], R * GN_RING);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = warp / W, in_row = warp % W, D = p.D;
   const uint32_t row_bytes = D * sizeof(T), gate_bytes = p.gate_f32 ? D * 4 : row_bytes;
-  const uint32_t stage_bytes = R * (4 * row_bytes + (G == GATE_FULL ? gate_bytes : 0));
-  const long long begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
-  const GnRing<R, 5> ring = {{static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.delta),
-                              static_cast<const uint8_t*>(p.dnormed), static_cast<const uint8_t*>(p.dsummed),
-                              G == GATE_FULL ? static_cast<const uint8_t*>(p.gate) : nullptr},
-                             {row_bytes, row_bytes, row_bytes, row_bytes, gate_bytes}, gn_smem, stage_bytes, p.stages, begin, R, end};
-  if (threadIdx.x == 0) ring.start(bars);
-  const int slot = warp / W, in_row = warp % W;
+  const uint32_t slot_bytes = 4 * row_bytes + (G == GATE_FULL ? gate_bytes : 0), stage_bytes = R * slot_bytes;
+  const int begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
+  const GnRing<5> ring = {{static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.delta),
+                           static_cast<const uint8_t*>(p.dnormed), static_cast<const uint8_t*>(p.dsummed),
+                           G == GATE_FULL ? static_cast<const uint8_t*>(p.gate) : nullptr},
+                          {row_bytes, row_bytes, row_bytes, row_bytes, gate_bytes}, gn_smem + slot * slot_bytes, stage_bytes,
+                          p.stages, bars[slot], begin + slot, R, end};
+  const bool leader = in_row == 0 && lane == 0;
+  if (leader) ring.start();
   const float inv = 1.f / D;
   float gwd[V][8], dw[V][8], a[V][8];                // a: dw_d, or the sum of dS nhat where rows share the gate
   if (G != GATE_SEQUENCE) load_gwd<T, W, G>(p, 0, in_row, lane, gwd);
@@ -665,32 +672,29 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
   int stage = 0, turn = 0;
   uint32_t phase = 0;
   bool here = true;
-  int sequence = -1;
-  for (long long block = begin; block < end; block += R, ++turn) {
-    const long long row = block + slot, at = row * D;
-    const bool live = row < end;
-    if (G == GATE_SEQUENCE && live && static_cast<int>(row) / p.seq != sequence) {
-      sequence = static_cast<int>(row) / p.seq;
+  int sequence = 0, sequence_end = 0;
+  for (int row = begin + slot; row < end; row += R, ++turn) {
+    const size_t at = static_cast<size_t>(row) * D;
+    if (G == GATE_SEQUENCE && row >= sequence_end) {
+      sequence = row / p.seq;
+      sequence_end = (sequence + 1) * p.seq;
       load_gwd<T, W, G>(p, row, in_row, lane, gwd);
     }
-    const float rd = live ? p.delta_rstd[row] : 0.f, r = live ? p.rstd[row] : 0.f;
-    const float token = G == GATE_TOKEN && live
+    const float rd = p.delta_rstd[row], r = p.rstd[row];
+    const float token = G == GATE_TOKEN
                             ? (p.gate_f32 ? static_cast<const float*>(p.gate)[row] : to_f32<T>(static_cast<const T*>(p.gate)[row]))
                             : 1.f;
-    const uint8_t* const x_row = gn_smem + stage * stage_bytes + slot * row_bytes;
-    const uint8_t* const d_row = x_row + R * row_bytes;
-    const uint8_t* const dy_row = d_row + R * row_bytes;
-    const uint8_t* const ds_row = dy_row + R * row_bytes;
-    const uint8_t* const g_row = gn_smem + stage * stage_bytes + 4 * R * row_bytes + slot * gate_bytes;
-    gn_arrived(here, bars.full[stage], phase, p.status, lane);
+    const uint8_t* const x_row = gn_smem + stage * stage_bytes + slot * slot_bytes;
+    const uint8_t *const d_row = x_row + row_bytes, *const dy_row = d_row + row_bytes, *const ds_row = dy_row + row_bytes;
+    const uint8_t* const g_row = ds_row + row_bytes;
+    gn_arrived(here, bars[slot][stage], phase, p.status, lane);
+    const float x_factor = p.residual_scale * r, d_factor = (G == GATE_TOKEN ? rd * token : rd) * r;
     float hat[V][8];                                   // of the sum, then dn w_d
     float sum = 0.f;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const int col = ((c * W + in_row) * 32 + lane) * 8;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) hat[c][i] = 0.f;
-      if (!live || col >= D) continue;
+      if (col >= D) continue;
       float d[8], x[8];
       ring_load<T>(x_row, col, x);
       ring_load<T>(d_row, col, d);
@@ -701,9 +705,8 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[i] *= g[i];
       }
-      const float factor = G == GATE_TOKEN ? rd * token : rd;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) hat[c][i] = (x[i] * p.residual_scale + d[i] * factor * gwd[c][i]) * r;
+      for (int i = 0; i < 8; ++i) hat[c][i] = x[i] * x_factor + d[i] * d_factor * gwd[c][i];
       if (p.dnormed) {
         float dy[8], w[8];
         ring_load<T>(dy_row, col, dy);
@@ -716,13 +719,13 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
         }
       }
     }
-    const float mean = gn_row_sum<W>(sum, scratch[0], slot, in_row, lane) * inv;
+    const float mean = gn_row_sum<W>(sum, scratch[0], slot, in_row, lane) * inv * r;
     Eight<T> dr[V];
     sum = 0.f;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const int col = ((c * W + in_row) * 32 + lane) * 8;
-      if (!live || col >= D) continue;
+      if (col >= D) continue;
       float d[8], ds[8], out[8];
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
@@ -736,7 +739,7 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
         ring_load<T>(dy_row, col, dy);
         load_w(c, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ds[i] += r * (dy[i] * w[i] - hat[c][i] * mean);
+        for (int i = 0; i < 8; ++i) ds[i] += dy[i] * w[i] * r - hat[c][i] * mean;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = ds[i] * p.residual_scale;
@@ -750,13 +753,14 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float nhat = d[i] * rd, part = ds[i] * nhat;
+        const float nhat = d[i] * rd;
         if (G == GATE_FULL) {
+          const float part = ds[i] * nhat;
           out[i] = part * gwd[c][i];                               // dS n
           a[c][i] += part * g[i];
           hat[c][i] = ds[i] * gwd[c][i] * g[i];
         } else {
-          a[c][i] += G == GATE_TOKEN ? part * token : part;
+          a[c][i] += G == GATE_TOKEN ? ds[i] * nhat * token : ds[i] * nhat;
           hat[c][i] = ds[i] * gwd[c][i];                           // the token's gate follows with the mean
         }
         sum += hat[c][i] * nhat;
@@ -772,20 +776,18 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
         }
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars.empty[stage]);
+    const int read = stage;
     if (++stage == p.stages) {
       stage = 0;
       phase ^= 1;
     }
     const float total = gn_row_sum<W>(sum, scratch[1], slot, in_row, lane);
-    if (threadIdx.x == 0) ring.refill(bars, R == 1 ? turn : turn - 1, p.status);
-    if (!live) continue;
-    if (G == GATE_TOKEN && in_row == 0 && lane == 0) {
+    if (leader) ring.refill(read, row);
+    if (G == GATE_TOKEN && leader) {
       if (p.gate_f32) static_cast<float*>(p.dgate)[row] = total;
       else static_cast<T*>(p.dgate)[row] = from_f32<T>(total);
     }
-    const float factor = G == GATE_TOKEN ? rd * token : rd, mean_d = total * inv * rd;
+    const float factor = G == GATE_TOKEN ? rd * token : rd, mean_d = total * inv * rd * factor;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const int col = ((c * W + in_row) * 32 + lane) * 8;
@@ -793,12 +795,12 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
       float d[8], out[8];
       dr[c].get(d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = factor * (hat[c][i] - d[i] * mean_d);
+      for (int i = 0; i < 8; ++i) out[i] = hat[c][i] * factor - d[i] * mean_d;
       Eight<T> e;
       e.set(out);
       e.store(static_cast<T*>(p.ddelta) + at, col, D, true);
     }
-    if (G == GATE_SEQUENCE && (row + R >= end || static_cast<int>(row + R) / p.seq != sequence)) {
+    if (G == GATE_SEQUENCE && row + R >= min(end, sequence_end)) {
       float* dst = sequences + (static_cast<long long>(sequence + blockIdx.x) * R + slot) * D;
 #pragma unroll
       for (int c = 0; c < V; ++c) {
@@ -824,59 +826,74 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
       for (int i = 0; i < 8; ++i) a[c][i] = dwd_smem[(c * 8 + i) * THREADS];
     }
   }
-  if (threadIdx.x == 0 && !here) ring.drain(bars, turn);
+  if (leader && !here) ring.drain(turn);
   // the ring's shared memory serves the sums: every copy has landed and been read
   gn_store_sums<R, W, THREADS>(p, dw, a, reinterpret_cast<float*>(gn_smem), slot, in_row, lane);
 }
 
-// Column sums of the partial rows: 32 columns per CTA, 16 partial rows at a time.  blockIdx.y: 0 dw; 1 dw_d, and the gradient of a
+// Column sums of the partial rows: VEC columns a thread, 16 partial rows at a time.  blockIdx.y: 0 dw; 1 dw_d, and the gradient of a
 // gate per channel; 2 + i the gradient of sequence i's gate.
+template <int VEC>
 __global__ void __launch_bounds__(512) gated_norm_sums_kernel(const GatedNormParams p, int ctas, int per_cta, int gate_bf16,
                                                               float* __restrict__ dw, float* __restrict__ dwd,
                                                               void* __restrict__ dgate) {
   chain_begin();
-  __shared__ float parts[16][33];
-  const int D = p.D, col = blockIdx.x * 32 + threadIdx.x;
+  __shared__ float parts[16][32 * VEC + 1];
+  const int D = p.D, col = (blockIdx.x * 32 + threadIdx.x) * VEC;
+  auto add = [&](float (&sum)[VEC], const float* src) {
+    if constexpr (VEC == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(src);
+      sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+    } else {
+      sum[0] += *src;
+    }
+  };
   for (long long what = blockIdx.y; what < 2 + (p.gate_kind == GATE_SEQUENCE ? p.rows / p.seq : 0); what += gridDim.y) {
-    float sum = 0.f;
-    if (what < 2) {
+    float sum[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+    if (what < 2 && col < D) {
       const float* src = p.partial + what * ctas * D + col;
-      if (col < D)
-        for (int r = threadIdx.y; r < ctas; r += 16) sum += src[static_cast<long long>(r) * D];
+#pragma unroll 4
+      for (int r = threadIdx.y; r < ctas; r += 16) add(sum, src + static_cast<long long>(r) * D);
     } else if (col < D) {
-      const long long i = what - 2, low = i * p.seq, high = low + p.seq;
-      const long long first = gn_cta_of(low, p.rows, ctas), last = gn_cta_of(high - 1, p.rows, ctas) + 1;
-      const float* src = p.partial + (2LL * ctas + i * per_cta) * D + col;
-      for (long long r = first * per_cta + threadIdx.y; r < last * per_cta; r += 16) {
+      const int i = static_cast<int>(what - 2), low = i * p.seq, high = low + p.seq;
+      const int first = gn_cta_of(low, p.rows, ctas), last = gn_cta_of(high - 1, p.rows, ctas) + 1;
+      const int base = p.rows / ctas, extra = p.rows % ctas;           // as gn_first_row
+      const float* src = p.partial + (2LL * ctas + static_cast<long long>(i) * per_cta) * D + col;
+      const int shift = 31 - __clz(per_cta);                           // a power of two
+      for (int r = (first << shift) + threadIdx.y; r < last << shift; r += 16) {
         // a slot that had none of the sequence's rows in this CTA has stored nothing
-        const long long cta = r / per_cta, begin = gn_first_row(cta, p.rows, ctas), end = gn_first_row(cta + 1, p.rows, ctas);
-        const long long from = low > begin ? low : begin, rows = (high < end ? high : end) - from;
-        if ((r + per_cta - (from - begin) % per_cta) % per_cta < rows) sum += src[r * D];
+        const int cta = r >> shift, begin = cta * base + min(cta, extra), end = begin + base + (cta < extra);
+        const int from = max(low, begin), rows = min(high, end) - from;
+        if ((r - (from - begin) & per_cta - 1) < rows) add(sum, src + static_cast<long long>(r) * D);
       }
     }
     __syncthreads();
-    parts[threadIdx.y][threadIdx.x] = sum;
-    __syncthreads();
-    if (threadIdx.y == 0 && col < D) {
-      sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum += parts[i][threadIdx.x];
+    for (int i = 0; i < VEC; ++i) parts[threadIdx.y][threadIdx.x * VEC + i] = sum[i];
+    __syncthreads();
+    const int column = threadIdx.y * 32 + threadIdx.x, at_col = blockIdx.x * 32 * VEC + column;
+    if (column < 32 * VEC && at_col < D) {
+      float total = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) total += parts[i][column];
       if (what == 0) {
-        dw[col] = sum;
+        dw[at_col] = total;
         continue;
       }
       if (what == 1) {
         float g = 1.f;
         if (p.gate_kind == GATE_CHANNEL) {
-          if (p.gate_f32) g = static_cast<const float*>(p.gate)[col];
-          else if (gate_bf16) g = __bfloat162float(static_cast<const __nv_bfloat16*>(p.gate)[col]);
-          else g = __half2float(static_cast<const __half*>(p.gate)[col]);
+          if (p.gate_f32) g = static_cast<const float*>(p.gate)[at_col];
+          else if (gate_bf16) g = __bfloat162float(static_cast<const __nv_bfloat16*>(p.gate)[at_col]);
+          else g = __half2float(static_cast<const __half*>(p.gate)[at_col]);
         }
-        dwd[col] = sum * g;
+        dwd[at_col] = total * g;
         if (p.gate_kind != GATE_CHANNEL) continue;
       }
-      const long long at = (what >= 2 ? what - 2 : 0) * D + col;
-      const float v = sum * p.delta_weight[col];
+      const long long at = (what >= 2 ? what - 2 : 0) * D + at_col;
+      const float v = total * p.delta_weight[at_col];
       if (p.gate_f32) static_cast<float*>(dgate)[at] = v;
       else if (gate_bf16) static_cast<__nv_bfloat16*>(dgate)[at] = __float2bfloat16(v);
       else static_cast<__half*>(dgate)[at] = __float2half(v);
@@ -973,8 +990,10 @@ static cudaError_t gn_launch(GatedNormParams& p, int type, bool backward, int ga
   }
   if (r != cudaSuccess) return r;
   const long long sums = 2 + (p.gate_kind == GATE_SEQUENCE ? p.rows / p.seq : 0);
-  return launch_next(gated_norm_sums_kernel, dim3((p.D + 31) / 32, static_cast<unsigned>(sums < 32768 ? sums : 32768)),
-                     dim3(32, 16), 0, s, p, ctas, R, gate_bf16, dw, dwd, p.dgate);
+  const unsigned y = static_cast<unsigned>(sums < 32768 ? sums : 32768);
+  if (p.aligned)
+    return launch_next(gated_norm_sums_kernel<4>, dim3((p.D + 127) / 128, y), dim3(32, 16), 0, s, p, ctas, R, gate_bf16, dw, dwd, p.dgate);
+  return launch_next(gated_norm_sums_kernel<1>, dim3((p.D + 31) / 32, y), dim3(32, 16), 0, s, p, ctas, R, gate_bf16, dw, dwd, p.dgate);
 }
 
 template <typename T>

@@ -25,90 +25,135 @@ namespace b2 {
 constexpr float E4M3_MAX = 448.f;
 constexpr float SMALLEST_SCALE = 7.52316384526264e-37f;     // 2^-120
 constexpr int F8_BM = 128, F8_BK = 128;
-constexpr int F8_THREADS = 320;
+constexpr int F8_EPI_WARPS = 8, F8_THREADS = 128 + 32 * F8_EPI_WARPS;
+// Registers: 384 threads x 168 at launch = 128 x 40 + 256 x 232 afterwards.
+constexpr int F8_FEW = 40, F8_MANY = 232;
 constexpr int F8_GROUP_M = 8;
-constexpr int F8_STAGING = 32 * 1024;
+constexpr int F8_AHEAD = 4;
+constexpr int F8_STAGING = F8_EPI_WARPS * 2048;
 
 // ------------------------------------------------------------------ quantisation
 enum QuantType : int { QUANT_F32 = 0, QUANT_BF16 = 1, QUANT_F16 = 2 };
 
-// 8 values of a row from column ``col`` on, zeros behind the last column.
-__device__ __forceinline__ void load8(const void* x, int type, long long at, int left, bool aligned, float (&f)[8]) {
-  if (aligned && left >= 8) {
-    if (type == QUANT_F32) {
-      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
-      const float4 a = src[0], b = src[1];
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-      const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 t = type == QUANT_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]))
-                                            : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        f[2 * i] = t.x;
-        f[2 * i + 1] = t.y;
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    f[i] = 0.f;
-    if (i < left) {
-      if (type == QUANT_F32) f[i] = static_cast<const float*>(x)[at + i];
-      else if (type == QUANT_BF16) f[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(x)[at + i]);
-      else f[i] = __half2float(static_cast<const __half*>(x)[at + i]);
-    }
-  }
-}
+template <typename T> __device__ __forceinline__ float quant_f32(T v);
+template <> __device__ __forceinline__ float quant_f32(float v) { return v; }
+template <> __device__ __forceinline__ float quant_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float quant_f32(__half v) { return __half2float(v); }
 
-// Values behind ``left`` are zero and stored too where they belong to the row's pitch.
-__device__ __forceinline__ void store8(uint8_t* q, float scale, const float (&f)[8]) {
+// 8 values of a row from ``x`` on, zeros behind the ``left`` that there are; as they are stored, which takes fewer registers.
+template <typename T>
+struct Values8 {
+  alignas(16) T v[8];
+  __device__ __forceinline__ void load(const T* x, int left, bool aligned) {
+    if (aligned && left >= 8) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(v) / 16); ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(x)[i];
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? x[i] : T(0.f);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = quant_f32<T>(v[i]);
+  }
+};
+
+// x / scale of a block, correctly rounded: a product with the rounded reciprocal and one correction by its remainder (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor", 1990), three operations a value where a
+// division is about ten.  Scales that are infinite, or so small that a remainder would underflow, are divided by.
+struct BlockScale {
+  float scale, inverse;
+  bool plain;
+};
+__device__ __forceinline__ BlockScale block_scale(float most) {
+  BlockScale s;
+  s.scale = fmaxf(most / E4M3_MAX, SMALLEST_SCALE);
+  s.inverse = 1.f / s.scale;
+  s.plain = !(s.scale > 1e-29f && s.scale < 1e36f);
+  return s;
+}
+__device__ __forceinline__ float scaled(float x, const BlockScale& s) {
+  const float first = x * s.inverse;
+  return __fmaf_rn(__fmaf_rn(-first, s.scale, x), s.inverse, first);
+}
+// Values behind the last column are zero and stored too where they belong to the row's pitch.
+template <typename T>
+__device__ __forceinline__ void store8(uint8_t* q, const BlockScale& s, const Values8<T>& x) {
+  float v[8], f[8];
+  x.get(f);
+  if (s.plain) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f[i] / s.scale;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = scaled(f[i], s);
+  }
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const __nv_fp8x2_storage_t a = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] / scale, f[4 * i + 1] / scale), __NV_SATFINITE, __NV_E4M3);
-    const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2] / scale, f[4 * i + 3] / scale), __NV_SATFINITE, __NV_E4M3);
-    w[i] = static_cast<uint32_t>(a) | static_cast<uint32_t>(b) << 16;
+    const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+    w[i] = a | b << 16;
   }
   *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
 }
 
 // NaN is passed over here; its value stays NaN.  Infinity makes the scale infinite and its own value NaN.
-__device__ __forceinline__ float largest8(const float (&f)[8]) {
-  float m = 0.f;
+template <typename T>
+__device__ __forceinline__ float largest8(const Values8<T>& x) {
+  float f[8], m = 0.f;
+  x.get(f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
   return m;
 }
 
-// One scale for 128 values of a row: half a warp per block, 8 values a lane.  ``pitch`` is a multiple of 16 and the row is filled with
-// zeros up to it.  Bound by memory traffic.
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int type, uint8_t* __restrict__ q,
-                                                            float* __restrict__ scales, long long M, int K, long long ldx,
+// One scale for 128 values of a row: eight lanes per block with 8 values of each half of it; a CTA has 64 consecutive blocks, 32
+// where there are few.  ``pitch`` is a multiple of 16 and the row is filled with zeros up to it.  Bound by memory traffic.
+template <typename T, int AHEAD>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                            float* __restrict__ scales, int M, int K, long long ldx,
                                                             long long pitch, long long scale_pitch, int aligned) {
   chain_begin();
-  const int lane16 = threadIdx.x & 15;
-  const long long blocks = (K + 127) / 128, total = M * blocks;
-  for (long long b = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 4; b < total;
-       b += static_cast<long long>(gridDim.x) * 16) {
-    const long long row = b / blocks;
-    const int kb = static_cast<int>(b - row * blocks), col = kb * 128 + lane16 * 8;
-    float f[8];
-    load8(x, type, row * ldx + col, K - col, aligned, f);
-    float m = largest8(f);
-    const unsigned mask = 0xffffu << (threadIdx.x & 16);
+  const int lane8 = threadIdx.x & 7, blocks = (K + 127) / 128;
+  const long long total = static_cast<long long>(M) * blocks;
+  const long long first = static_cast<long long>(blockIdx.x) * 32 * AHEAD + (threadIdx.x >> 3);
+  Values8<T> f[AHEAD][2];
+  int row[AHEAD], kb[AHEAD];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, o));
-    const float scale = fmaxf(m / E4M3_MAX, SMALLEST_SCALE);
-    if (col < pitch) store8(q + row * pitch + col, scale, f);
-    if (lane16 == 0) scales[kb * scale_pitch + row] = scale;
+  for (int i = 0; i < AHEAD; ++i) {
+    const long long b = first + i * 32;
+    if (total <= 0x7fffffffLL) {
+      row[i] = static_cast<int>(b) / blocks;
+      kb[i] = static_cast<int>(b) - row[i] * blocks;
+    } else {
+      row[i] = static_cast<int>(b / blocks);
+      kb[i] = static_cast<int>(b - static_cast<long long>(row[i]) * blocks);
+    }
+    const int col = kb[i] * 128 + lane8 * 8;
+    const T* src = x + row[i] * ldx + col;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) f[i][h].load(src + 64 * h, b < total ? K - col - 64 * h : 0, aligned);
+  }
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    float m = fmaxf(largest8(f[i][0]), largest8(f[i][1]));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (first + i * 32 >= total) continue;
+    const BlockScale s = block_scale(m);
+    const int col = kb[i] * 128 + lane8 * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (col + 64 * h < pitch) store8(q + row[i] * pitch + col + 64 * h, s, f[i][h]);
+    if (lane8 == 0) scales[kb[i] * scale_pitch + row[i]] = s.scale;
   }
 }
 
 // One scale for 128 x 128 values: a CTA per block, 64 values a thread.
-__global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __restrict__ x, int type, uint8_t* __restrict__ q,
+template <typename T>
+__global__ void __launch_bounds__(256, 3) quantize_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                               float* __restrict__ scales, int M, int K, long long ldx,
                                                               long long pitch, int aligned) {
   chain_begin();
@@ -116,13 +161,15 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __rest
   const int kb = blockIdx.x, lane16 = threadIdx.x & 15, col = kb * 128 + lane16 * 8;
   for (long long mb = blockIdx.y; mb * 128 < M; mb += gridDim.y) {
     const long long row0 = mb * 128 + (threadIdx.x >> 4);
-    float f[8][8], m = 0.f;
+    Values8<T> f[8];
+    float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const long long row = row0 + i * 16;
-      load8(x, type, row * ldx + col, row < M ? K - col : 0, aligned, f[i]);
-      m = fmaxf(m, largest8(f[i]));
+      f[i].load(x + row * ldx + col, row < M ? K - col : 0, aligned);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, largest8(f[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     __syncthreads();
@@ -130,13 +177,13 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __rest
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = fmaxf(m, most[i]);
-    const float scale = fmaxf(m / E4M3_MAX, SMALLEST_SCALE);
+    const BlockScale s = block_scale(m);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const long long row = row0 + i * 16;
-      if (row < M && col < pitch) store8(q + row * pitch + col, scale, f[i]);
+      if (row < M && col < pitch) store8(q + row * pitch + col, s, f[i]);
     }
-    if (threadIdx.x == 0) scales[mb * gridDim.x + kb] = scale;
+    if (threadIdx.x == 0) scales[mb * gridDim.x + kb] = s.scale;
   }
 }
 
@@ -158,19 +205,6 @@ template <int BN> struct F8Cfg {
   static constexpr int SLOTS = 512 / BN < 4 ? 512 / BN : 4;      // accumulators in tensor memory
   static constexpr int SMEM = STAGES * STAGE_BYTES + F8_STAGING + 1024 + 256;
 };
-
-// d += s * v for two values at a time.
-__device__ __forceinline__ void fma2(uint64_t& d, uint32_t lo, uint32_t hi, uint64_t s) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(v), "l"(s));
-}
-__device__ __forceinline__ void split2(uint64_t d, float& lo, float& hi) {
-  uint32_t a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(d));
-  lo = __uint_as_float(a);
-  hi = __uint_as_float(b);
-}
 
 // SPLIT: the CTAs of a cluster share a tile, each has a run of its blocks along k; their sums meet in the order of the CTAs through
 // the cluster's shared memory.
@@ -194,7 +228,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
     }
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&tmem_full[s], 1);
-      mbar_init(&tmem_empty[s], 8);
+      mbar_init(&tmem_empty[s], F8_EPI_WARPS);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -224,9 +258,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
     n0 = in_group / rows * BN;
   };
 
-  if (warp == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8_FEW));
     // ------------------------------------------------------------ TMA producer
-    if (elect_one()) {
+    if (warp == 0 && elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       bool wrapped = false;
@@ -262,9 +297,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
           if (wrapped || s < stage) mbar_wait(&full_bar[s], s < stage ? phase : phase ^ 1);
       }
     }
-  } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (elect_one()) {
+    if (warp == 1 && elect_one()) {
       constexpr uint32_t idesc = umma_idesc_e4m3(F8_BM, BN, B_MN);
       int stage = 0, slot = 0;
       uint32_t phase = 0, slot_phase = 0;
@@ -297,10 +331,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
       }
     }
   } else {
-    // ------------------------------------------------------------ scales, sums and stores (eight warps)
-    const int quad = warp & 3, half = (warp - 2) >> 2;       // TMEM lanes and column half of this warp
-    uint4* const staged = reinterpret_cast<uint4*>(smem + STAGES * C::STAGE_BYTES) + (warp - 2) * 256;
-    auto swz = [](int r) { return (r & 1) | ((r & 2) << 1) | ((r & 4) >> 1); };
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_MANY));
+    // ------------------------------------------------------------ scales, sums and stores
+    const int quad = warp & 3, part_of_n = (warp - 4) >> 2;  // TMEM lanes and columns of this warp
+    uint4* const staged = reinterpret_cast<uint4*>(smem + STAGES * C::STAGE_BYTES) + (warp - 4) * 128;
+    constexpr int STEP = COLS < 32 ? COLS : 32;              // columns at a time
     int slot = 0;
     uint32_t slot_phase = 0;
     const bool vectors = p.N % 8 == 0;
@@ -309,44 +344,56 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
       place(tile, m0, n0);
       const int row = m0 + quad * 32 + lane;
       const float* a_scale = p.a_scales + min(row, p.M - 1) * p.a_row;
-      // a column half behind the last column has no scale; its sums are not stored
-      const float* b_scale = p.b_scales + (min(n0 + half * COLS, p.N - 1) / 128) * p.b_row;
-      uint64_t acc[COLS / 2];
+      // columns behind the last one have no scale; their sums are not stored
+      const float* b_scale = p.b_scales + (min(n0 + part_of_n * COLS, p.N - 1) / 128) * p.b_row;
+      float acc[COLS];
 #pragma unroll
-      for (int i = 0; i < COLS / 2; ++i) acc[i] = 0;
-      float sa = 0.f, sb = 0.f;
-      if (kb_begin < kb_end) {
-        sa = a_scale[kb_begin * p.a_block];
-        sb = b_scale[kb_begin * p.b_block];
+      for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
+      // the scales of the next F8_AHEAD blocks are on their way: an access to a far part of L2 takes longer than a block
+      float sa[F8_AHEAD], sb[F8_AHEAD];
+#pragma unroll
+      for (int i = 0; i < F8_AHEAD; ++i) {
+        const bool there = kb_begin + i < kb_end;
+        sa[i] = there ? a_scale[(kb_begin + i) * p.a_block] : 0.f;
+        sb[i] = there ? b_scale[(kb_begin + i) * p.b_block] : 0.f;
       }
       for (int kb = kb_begin; kb < kb_end; ++kb) {
-        const float s = sa * sb;
-        if (kb + 1 < kb_end) {
-          sa = a_scale[(kb + 1) * p.a_block];
-          sb = b_scale[(kb + 1) * p.b_block];
+        const float s = sa[0] * sb[0];
+#pragma unroll
+        for (int i = 0; i + 1 < F8_AHEAD; ++i) {
+          sa[i] = sa[i + 1];
+          sb[i] = sb[i + 1];
         }
-        uint64_t s2;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "r"(__float_as_uint(s)));
+        if (kb + F8_AHEAD < kb_end) {
+          sa[F8_AHEAD - 1] = a_scale[(kb + F8_AHEAD) * p.a_block];
+          sb[F8_AHEAD - 1] = b_scale[(kb + F8_AHEAD) * p.b_block];
+        }
         if (!mbar_wait(&tmem_full[slot], slot_phase)) {
           *abort_flag = 1;
           atomicExch(p.status, 4);
           break;
         }
         tc_fence_after();
-        const uint32_t taddr = tmem_base + slot * BN + half * COLS + (static_cast<uint32_t>(quad * 32) << 16);
-        uint32_t v[2][16];
-        tmem_ld_32x16(taddr, v[0]);
+        const uint32_t taddr = tmem_base + slot * BN + part_of_n * COLS + (static_cast<uint32_t>(quad * 32) << 16);
+        // Up to 64 columns at a time: a load from tensor memory takes longer than the additions of 32, and the other warp of the
+        // scheduler adds meanwhile.
+        constexpr int WIDE = COLS < 64 ? COLS : 64;
 #pragma unroll
-        for (int c = 0; c < COLS / 16; ++c) {
+        for (int c = 0; c < COLS; c += WIDE) {
+          uint32_t v[WIDE / STEP][STEP];
+#pragma unroll
+          for (int h = 0; h < WIDE / STEP; ++h) {
+            if constexpr (STEP == 32) tmem_ld_32x32(taddr + c + h * STEP, v[h]);
+            else tmem_ld_32x16(taddr + c + h * STEP, v[h]);
+          }
           tmem_ld_wait();
-          if (c + 1 < COLS / 16) tmem_ld_32x16(taddr + (c + 1) * 16, v[(c + 1) & 1]);
-          else {
+          if (c + WIDE == COLS) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tmem_empty[slot]);
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], s2);
+          for (int i = 0; i < WIDE; ++i) acc[c + i] = __fmaf_rn(__uint_as_float(v[i / STEP][i % STEP]), s, acc[c + i]);
         }
         if (++slot == SLOTS) {
           slot = 0;
@@ -357,38 +404,29 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
         // [column][row] of this CTA's part, in the shared memory of its operands, which have been read
         float* mine = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int i = 0; i < COLS / 2; ++i) {
-          float lo, hi;
-          split2(acc[i], lo, hi);
-          mine[(half * COLS + 2 * i) * F8_BM + quad * 32 + lane] = lo;
-          mine[(half * COLS + 2 * i + 1) * F8_BM + quad * 32 + lane] = hi;
-        }
+        for (int i = 0; i < COLS; ++i) mine[(part_of_n * COLS + i) * F8_BM + quad * 32 + lane] = acc[i];
         break;                                       // one tile per cluster
       }
-      // 64 columns of 32 rows at a time through shared memory, so that a row leaves in 128 contiguous bytes
+      // STEP columns of 32 rows at a time through shared memory (16-byte units, swizzled), so that a row leaves in 64 contiguous bytes
+      constexpr int UNITS = STEP / 8;
 #pragma unroll
-      for (int c = 0; c < COLS; c += 64) {
-        const int col0 = n0 + half * COLS + c;
+      for (int c = 0; c < COLS; c += STEP) {
+        const int col0 = n0 + part_of_n * COLS + c;
         if (col0 >= p.N) break;
-        constexpr int WIDE = COLS < 64 ? COLS : 64;
 #pragma unroll
-        for (int i = 0; i < WIDE / 8; ++i) {
+        for (int i = 0; i < UNITS; ++i) {
           uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float lo, hi;
-            split2(acc[c / 2 + i * 4 + k], lo, hi);
-            w[k] = pack_bf16(lo, hi);
-          }
-          staged[lane * 8 + (i ^ swz(lane))] = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int k = 0; k < 4; ++k) w[k] = pack_bf16(acc[c + i * 8 + 2 * k], acc[c + i * 8 + 2 * k + 1]);
+          staged[lane * 4 + (i ^ (lane >> 1 & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         __syncwarp();
-        const int unit = lane & 7, col = col0 + unit * 8;
+        const int unit = lane & 3, col = col0 + unit * 8;
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int r = it * 4 + (lane >> 3), out_row = m0 + quad * 32 + r;
-          if (out_row >= p.M || unit * 8 >= WIDE || col >= p.N) continue;
-          const uint4 v = staged[r * 8 + (unit ^ swz(r))];
+        for (int it = 0; it < 4; ++it) {
+          const int r = it * 8 + (lane >> 2), out_row = m0 + quad * 32 + r;
+          if (out_row >= p.M || unit >= UNITS || col >= p.N) continue;
+          const uint4 v = staged[r * 4 + (unit ^ (r >> 1 & 3))];
           __nv_bfloat16* dst = p.d + static_cast<long long>(out_row) * p.N + col;
           if (vectors) {
             *reinterpret_cast<uint4*>(dst) = v;
@@ -477,6 +515,25 @@ static int launch_fp8(const Fp8Params& p, cudaStream_t s) {
   return 0;
 }
 
+template <typename T>
+static cudaError_t launch_quantize(const void* x, void* q, float* scales, int M, int K, long long ldx, long long pitch,
+                                   long long scale_pitch, int block_rows, int aligned, cudaStream_t s) {
+  const T* in = static_cast<const T*>(x);
+  uint8_t* out = static_cast<uint8_t*>(q);
+  const long long across = (K + 127) / 128, blocks = M * across;
+  if (block_rows == 128) {
+    const long long rows = (M + 127) / 128;
+    return launch_next(quantize_blocks_kernel<T>, dim3(static_cast<unsigned>(across), static_cast<unsigned>(rows < 32768 ? rows : 32768)),
+                       256, 0, s, in, out, scales, M, K, ldx, pitch, aligned);
+  }
+  // few blocks are spread over more CTAs
+  if (blocks <= f8_sms() * 64LL)
+    return launch_next(quantize_rows_kernel<T, 1>, static_cast<unsigned>((blocks + 31) / 32), 256, 0, s, in, out, scales, M, K, ldx,
+                       pitch, scale_pitch, aligned);
+  return launch_next(quantize_rows_kernel<T, 2>, static_cast<unsigned>((blocks + 63) / 64), 256, 0, s, in, out, scales, M, K, ldx,
+                     pitch, scale_pitch, aligned);
+}
+
 }  // namespace b2
 
 using namespace b2;
@@ -493,16 +550,11 @@ int b2_quantize_fp8(const void* x, int type, void* q, float* scales, long long M
   if (M == 0) return 0;
   const int size = type == QUANT_F32 ? 4 : 2;
   const int aligned = ldx * size % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  cudaError_t r;
-  if (block_rows == 1) {
-    const long long ctas = (M * ((K + 127) / 128) + 15) / 16, most = f8_sms() * 8LL;
-    r = launch_next(quantize_rows_kernel, static_cast<unsigned>(ctas < most ? ctas : most), 256, 0, s, x, type,
-                    static_cast<uint8_t*>(q), scales, M, K, ldx, pitch, scale_pitch, aligned);
-  } else {
-    const long long rows = (M + 127) / 128;
-    r = launch_next(quantize_blocks_kernel, dim3((K + 127) / 128, static_cast<unsigned>(rows < 32768 ? rows : 32768)), 256, 0, s, x,
-                    type, static_cast<uint8_t*>(q), scales, static_cast<int>(M), K, ldx, pitch, aligned);
-  }
+  const int rows = static_cast<int>(M);
+  const cudaError_t r =
+      type == QUANT_F32    ? launch_quantize<float>(x, q, scales, rows, K, ldx, pitch, scale_pitch, block_rows, aligned, s)
+      : type == QUANT_BF16 ? launch_quantize<__nv_bfloat16>(x, q, scales, rows, K, ldx, pitch, scale_pitch, block_rows, aligned, s)
+                           : launch_quantize<__half>(x, q, scales, rows, K, ldx, pitch, scale_pitch, block_rows, aligned, s);
   if (r != cudaSuccess) cudaGetLastError();
   return r == cudaSuccess ? 0 : -1;
 }

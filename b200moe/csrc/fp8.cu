@@ -8,9 +8,12 @@
 // 128 x 128 block has the same scale either way.
 //
 // Product.  The tensor cores add up one block of 128 (four instructions of 32) in an accumulator of its own; the warps of the
-// epilogue multiply it by the two scales and add it to fp32 registers, while the next blocks are in flight: accumulators of
-// 512 / BN blocks fit in tensor memory.  A tile of 128 x 256 has 128 sums per thread of eight warps.  A block of such a tile takes
-// the tensor cores 512 cycles and the epilogue one fused multiply-add per value, 128 for each pair of lanes.
+// epilogue multiply it by the two scales, which two warps form ahead, and add it to fp32 registers, while the next blocks are in
+// flight: accumulators of 512 / BN blocks fit in tensor memory.  A block of a 128 x 256 tile is 768 cycles of shared memory (48 KiB
+// written by TMA and read by the tensor cores, which would need 512), and one fused multiply-add per value, 256 issue slots of each
+// scheduler.  Large products run against the power limit: 16384 x 6144, K 4096 takes 408 us (2.0 PFLOP/s, bf16 520 us), without the
+// additions 320 us at a lower clock.  Pairs of CTAs (cta_group::2), which halve the traffic of B, were slower (616 us): an accumulator
+// goes back and forth between two CTAs for every block.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -26,8 +29,8 @@ constexpr float E4M3_MAX = 448.f;
 constexpr float SMALLEST_SCALE = 7.52316384526264e-37f;     // 2^-120
 constexpr int F8_BM = 128, F8_BK = 128;
 constexpr int F8_EPI_WARPS = 8, F8_THREADS = 128 + 32 * F8_EPI_WARPS;
-// Registers: 384 threads x 168 at launch = 128 x 40 + 256 x 232 afterwards.
-constexpr int F8_FEW = 40, F8_MANY = 232;
+// Registers: 384 threads x 168 at launch = 128 x 72 + 256 x 216 afterwards.
+constexpr int F8_FEW = 72, F8_MANY = 216;
 constexpr int F8_GROUP_M = 8;
 constexpr int F8_AHEAD = 4;
 constexpr int F8_STAGING = F8_EPI_WARPS * 2048;
@@ -203,7 +206,7 @@ template <int BN> struct F8Cfg {
   static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
   static constexpr int A_BYTES = F8_BM * F8_BK, B_BYTES = BN * F8_BK, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int SLOTS = 512 / BN < 4 ? 512 / BN : 4;      // accumulators in tensor memory
-  static constexpr int SMEM = STAGES * STAGE_BYTES + F8_STAGING + 1024 + 256;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + F8_STAGING + 1024 /*align*/ + 256 /*barriers*/ + SLOTS * 1024 /*scales*/;
 };
 
 // SPLIT: the CTAs of a cluster share a tile, each has a run of its blocks along k; their sums meet in the order of the CTAs through
@@ -220,6 +223,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
   uint64_t* tmem_empty = tmem_full + SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + SLOTS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* const scale_smem = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES + F8_STAGING + 256);      // [slot][column half][row]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
       mbar_init(&empty_bar[s], 1);
     }
     for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(&tmem_full[s], 1);
+      mbar_init(&tmem_full[s], 1 + 2);         // the products, and the scales of two warps
       mbar_init(&tmem_empty[s], F8_EPI_WARPS);
     }
     *abort_flag = 0;
@@ -330,6 +334,51 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
         }
       }
     }
+    // ------------------------------------------------------------ scales (two warps, two rows a thread)
+    // The products of both scales of each row and column half go to shared memory beside the accumulator that they belong to.  Those
+    // of the next F8_AHEAD blocks are on their way: an access to a far part of L2 takes longer than a block.
+    if (warp >= 2) {
+      const int r = (warp - 2) * 64 + lane * 2;
+      int slot = 0;
+      uint32_t slot_phase = 1;
+      for (long long tile = worker; tile < tiles && !*abort_flag; tile += workers) {
+        int m0, n0;
+        place(tile, m0, n0);
+        const float* const a0 = p.a_scales + min(m0 + r, p.M - 1) * p.a_row;
+        const float* const a1 = p.a_scales + min(m0 + r + 1, p.M - 1) * p.a_row;
+        // columns behind the last one have no scale; their sums are not stored
+        const float* const b0 = p.b_scales + (min(n0, p.N - 1) / 128) * p.b_row;
+        const float* const b1 = p.b_scales + (min(n0 + BN / 2, p.N - 1) / 128) * p.b_row;
+        float4 ahead[F8_AHEAD];
+        auto fetch = [&](int kb) {
+          return kb < kb_end ? make_float4(a0[kb * p.a_block], a1[kb * p.a_block], b0[kb * p.b_block], b1[kb * p.b_block])
+                             : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+#pragma unroll
+        for (int i = 0; i < F8_AHEAD; ++i) ahead[i] = fetch(kb_begin + i);
+        for (int kb0 = kb_begin; kb0 < kb_end && !*abort_flag; kb0 += F8_AHEAD) {
+#pragma unroll
+          for (int i = 0; i < F8_AHEAD; ++i) {       // unrolled: a value that moved to another register would be waited for
+            if (kb0 + i >= kb_end) break;
+            const float4 v = ahead[i];
+            ahead[i] = fetch(kb0 + i + F8_AHEAD);
+            if (!mbar_wait(&tmem_empty[slot], slot_phase)) {
+              *abort_flag = 1;
+              atomicExch(p.status, 3);
+              break;
+            }
+            *reinterpret_cast<float2*>(scale_smem + (slot * 2) * F8_BM + r) = make_float2(v.x * v.z, v.y * v.z);
+            *reinterpret_cast<float2*>(scale_smem + (slot * 2 + 1) * F8_BM + r) = make_float2(v.x * v.w, v.y * v.w);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tmem_full[slot]);
+            if (++slot == SLOTS) {
+              slot = 0;
+              slot_phase ^= 1;
+            }
+          }
+        }
+      }
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_MANY));
     // ------------------------------------------------------------ scales, sums and stores
@@ -342,58 +391,32 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
     for (long long tile = worker; tile < tiles && !*abort_flag; tile += workers) {
       int m0, n0;
       place(tile, m0, n0);
-      const int row = m0 + quad * 32 + lane;
-      const float* a_scale = p.a_scales + min(row, p.M - 1) * p.a_row;
-      // columns behind the last one have no scale; their sums are not stored
-      const float* b_scale = p.b_scales + (min(n0 + part_of_n * COLS, p.N - 1) / 128) * p.b_row;
       float acc[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
-      // the scales of the next F8_AHEAD blocks are on their way: an access to a far part of L2 takes longer than a block
-      float sa[F8_AHEAD], sb[F8_AHEAD];
-#pragma unroll
-      for (int i = 0; i < F8_AHEAD; ++i) {
-        const bool there = kb_begin + i < kb_end;
-        sa[i] = there ? a_scale[(kb_begin + i) * p.a_block] : 0.f;
-        sb[i] = there ? b_scale[(kb_begin + i) * p.b_block] : 0.f;
-      }
       for (int kb = kb_begin; kb < kb_end; ++kb) {
-        const float s = sa[0] * sb[0];
-#pragma unroll
-        for (int i = 0; i + 1 < F8_AHEAD; ++i) {
-          sa[i] = sa[i + 1];
-          sb[i] = sb[i + 1];
-        }
-        if (kb + F8_AHEAD < kb_end) {
-          sa[F8_AHEAD - 1] = a_scale[(kb + F8_AHEAD) * p.a_block];
-          sb[F8_AHEAD - 1] = b_scale[(kb + F8_AHEAD) * p.b_block];
-        }
         if (!mbar_wait(&tmem_full[slot], slot_phase)) {
           *abort_flag = 1;
           atomicExch(p.status, 4);
           break;
         }
         tc_fence_after();
+        const float s = scale_smem[(slot * 2 + part_of_n) * F8_BM + quad * 32 + lane];
         const uint32_t taddr = tmem_base + slot * BN + part_of_n * COLS + (static_cast<uint32_t>(quad * 32) << 16);
-        // Up to 64 columns at a time: a load from tensor memory takes longer than the additions of 32, and the other warp of the
-        // scheduler adds meanwhile.
-        constexpr int WIDE = COLS < 64 ? COLS : 64;
+        // (Two columns per instruction, which packed arithmetic has, are slower: 501 us against 440 at 16384 x 6144, K 4096.)
 #pragma unroll
-        for (int c = 0; c < COLS; c += WIDE) {
-          uint32_t v[WIDE / STEP][STEP];
-#pragma unroll
-          for (int h = 0; h < WIDE / STEP; ++h) {
-            if constexpr (STEP == 32) tmem_ld_32x32(taddr + c + h * STEP, v[h]);
-            else tmem_ld_32x16(taddr + c + h * STEP, v[h]);
-          }
+        for (int c = 0; c < COLS; c += STEP) {
+          uint32_t v[STEP];
+          if constexpr (STEP == 32) tmem_ld_32x32(taddr + c, v);
+          else tmem_ld_32x16(taddr + c, v);
           tmem_ld_wait();
-          if (c + WIDE == COLS) {
+          if (c + STEP == COLS) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tmem_empty[slot]);
           }
 #pragma unroll
-          for (int i = 0; i < WIDE; ++i) acc[c + i] = __fmaf_rn(__uint_as_float(v[i / STEP][i % STEP]), s, acc[c + i]);
+          for (int i = 0; i < STEP; ++i) acc[c + i] = __fmaf_rn(__uint_as_float(v[i]), s, acc[c + i]);
         }
         if (++slot == SLOTS) {
           slot = 0;
@@ -446,12 +469,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
     cluster_sync_all();
     int m0, n0;
     place(worker, m0, n0);
-    // this CTA's share of the columns; consecutive threads hold consecutive rows
+    // this CTA's share of the columns, two at a time; consecutive threads hold consecutive rows
     constexpr int SHARE = BN / (SPLIT ? SPLIT : 1);
     const bool bad = *abort_flag != 0;
-    for (int i = threadIdx.x; i < F8_BM * (SHARE / 2) && !bad; i += F8_THREADS) {
-      const int r = i % F8_BM, c = part * SHARE + i / F8_BM * 2;
-      if (m0 + r >= p.M || n0 + c >= p.N) continue;
+    const int rows = min(F8_BM, p.M - m0);
+    for (int i = threadIdx.x; i < rows * (SHARE / 2) && !bad; i += F8_THREADS) {
+      const int r = i % rows, c = part * SHARE + i / rows * 2;
+      if (n0 + c >= p.N) continue;
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < parts; ++k) {
@@ -515,6 +539,45 @@ static int launch_fp8(const Fp8Params& p, cudaStream_t s) {
   return 0;
 }
 
+// Tile width and split by a model of the time, in units of a block of a 256-column tile (0.6 us): waves of tiles, each with its blocks
+// along k and an end.  Fitted to, us of 256, 128 and 64 columns: 1003 x 4096, K 4096 20, 22, 36; 64 x 14336, K 4096 20, 11.5, 18; 2048
+// x 4096, K 1024 15, 15, 18; 128 x 512, K 512 5, 3, 2.  Few rows leave SMs without a tile: CTAs of a cluster share the blocks of one
+// (16 x 1024, K 14336, 128 columns: 29 us on one CTA a tile, 20, 11 and 7 on two, four and eight; 16 x 4096, K 4096 9.4, 9, 7 on
+// one, two and four).  Joining them costs by the row: 128 x 512, K 512 3 us alone, 13 shared by two.
+struct Fp8Choice {
+  int bn, split;
+};
+static Fp8Choice choose_fp8(int M, int N, int K, int nn) {
+  const long long rows = (M + F8_BM - 1) / F8_BM, blocks = (K + F8_BK - 1) / F8_BK, sms = f8_sms();
+  Fp8Choice best = {256, 0};
+  double least = 1e30;
+  for (int bn : {256, 128, 64}) {
+    if (nn && bn == 64) continue;                    // a box of B along its columns is 128 wide
+    const long long tiles = rows * ((N + bn - 1) / bn);
+    const double block = bn == 256 ? 1.0 : bn == 128 ? 0.55 : 0.46, end = bn == 256 ? 4.7 : bn == 128 ? 2.0 : 0.5;
+    for (int split : {1, 2, 4, 8}) {
+      // clusters that the device holds at a time, with a margin: they do not cross its partitions
+      if (split > 1 && (M > 32 || blocks < 2 * split || tiles > (split == 2 ? 70 : split == 4 ? 32 : 14))) continue;
+      const double time = (split > 1 ? 1 : (tiles + sms - 1) / sms) * ((blocks + split - 1) / split * block + end) + (split > 1 ? 3.0 : 0.0);
+      if (time < least) {
+        least = time;
+        best = {bn, split > 1 ? split : 0};
+      }
+    }
+  }
+  return best;
+}
+
+template <int BN, int B_MN>
+static int launch_fp8(const Fp8Params& p, int split, cudaStream_t s) {
+  switch (split) {
+    case 2: return launch_fp8<BN, B_MN, 2>(p, s);
+    case 4: return launch_fp8<BN, B_MN, 4>(p, s);
+    case 8: return launch_fp8<BN, B_MN, 8>(p, s);
+    default: return launch_fp8<BN, B_MN, 0>(p, s);
+  }
+}
+
 template <typename T>
 static cudaError_t launch_quantize(const void* x, void* q, float* scales, int M, int K, long long ldx, long long pitch,
                                    long long scale_pitch, int block_rows, int aligned, cudaStream_t s) {
@@ -570,9 +633,11 @@ int b2_gemm_fp8(const void* a, const float* a_scales, const void* w, const float
   p.a_scales = a_scales; p.b_scales = b_scales; p.a_row = a_row; p.a_block = a_block; p.b_row = b_row; p.b_block = b_block;
   p.d = static_cast<__nv_bfloat16*>(d); p.M = M; p.N = N; p.K = K; p.status = status;
   if (make_map8(&p.map_a, a, K, M, lda, F8_BM)) return -11;
-  const int bn = 256;
-  if (nn ? make_map8(&p.map_b, w, N, K, ldw, 128) : make_map8(&p.map_b, w, K, N, ldw, bn)) return -12;
-  return nn ? launch_fp8<256, 1, 0>(p, s) : launch_fp8<256, 0, 0>(p, s);
+  const Fp8Choice c = choose_fp8(M, N, K, nn);
+  if (nn ? make_map8(&p.map_b, w, N, K, ldw, 128) : make_map8(&p.map_b, w, K, N, ldw, c.bn)) return -12;
+  if (nn) return c.bn == 256 ? launch_fp8<256, 1>(p, c.split, s) : launch_fp8<128, 1>(p, c.split, s);
+  if (c.bn == 256) return launch_fp8<256, 0>(p, c.split, s);
+  return c.bn == 128 ? launch_fp8<128, 0>(p, c.split, s) : launch_fp8<64, 0>(p, c.split, s);
 }
 
 }  // extern "C"

@@ -320,7 +320,8 @@ def _check_product(got, a, b):
 
 @pytest.mark.parametrize("M,N,K", [(1, 16, 16), (1, 4096, 4096), (16, 4096, 2048), (17, 300, 1000), (128, 256, 128), (130, 129, 130),
                                    (200, 1000, 64), (257, 517, 513), (1003, 1544, 2000), (300, 8, 4096), (64, 64, 14336), (640, 4096, 384),
-                                   (129, 1, 77), (2500, 2000, 257), (5000, 320, 1024)])
+                                   (129, 1, 77), (2500, 2000, 257), (5000, 320, 1024), (16, 1024, 14336), (7, 520, 9000), (32, 2056, 4096),
+                                   (31, 136, 1031), (33, 4096, 4096)])
 def test_matmul_fp8(M, N, K):
     a, sa = _operand(M, K, 1)
     b, sb = _operand(N, K, 128)

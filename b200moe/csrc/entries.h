@@ -53,6 +53,24 @@ int b2_scale_bf16(void* x, const float* factor, long long n, cudaStream_t s);
 int b2_embedding_fwd(const long long* ids, const void* table, void* out, int T, int D, cudaStream_t s);
 int b2_embedding_bwd(const long long* ids, const void* dy, float* dtable, int T, int D, cudaStream_t s);
 int b2_moe_aux(const float* probs, const int* counts, float* aux, int T, int E, cudaStream_t s);
+// route.cu, gated_norm.cu, fp8.cu
+int b2_route_topk(const void* logits, const float* bias, float* weights, long long* idx, long long T, int E, int k, int type,
+                  int sigmoid, int groups, int top_groups, int two_best, int renormalize, float scale, cudaStream_t s);
+int b2_route_topk_bwd(const void* logits, const float* weights, const long long* idx, const float* dweights, void* dlogits,
+                      long long T, int E, int k, int type, int sigmoid, int renormalize, float scale, cudaStream_t s);
+int b2_gated_norm_fwd(const void* x, const void* delta, const float* delta_weight, const float* weight, const void* gate,
+                      void* summed, void* normed, float* delta_rstd, float* rstd, int rows, int D, int seq, int type,
+                      int gate_kind, int gate_f32, float residual_scale, float eps, int* status, cudaStream_t s);
+long long b2_gated_norm_bwd_floats(int rows, int D, int seq, int gate_kind);
+int b2_gated_norm_bwd(const void* dsummed, const void* dnormed, const void* x, const void* delta, const float* delta_weight,
+                      const float* weight, const void* gate, const float* delta_rstd, const float* rstd, void* dx, void* ddelta,
+                      float* dwd, float* dw, void* dgate, float* partial, int rows, int D, int seq, int type, int gate_kind,
+                      int gate_f32, float residual_scale, int* status, cudaStream_t s);
+int b2_quantize_fp8(const void* x, int type, void* q, float* scales, long long M, int K, long long ldx, long long pitch,
+                    long long scale_pitch, int block_rows, cudaStream_t s);
+int b2_gemm_fp8(const void* a, const float* a_scales, const void* w, const float* b_scales, void* d, int M, int N, int K,
+                long long lda, long long ldw, long long a_row, long long a_block, long long b_row, long long b_block, int nn,
+                int* status, cudaStream_t s);
 // layers.cu
 const char* b2_layers_refused();
 int b2_attn_half_fwd(const void* x, const float* ln1, const void* wqkv, const float* cos_t, const float* sin_t, const void* wo,

@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include "chain.cuh"
+#include "entries.h"
 #include "ptx.cuh"
 #include "tensormap.cuh"
 

@@ -1,12 +1,14 @@
-// Autograd nodes of the training step in C++: embedding, norm, the attention half of a block, the routed layer on one rank, and
-// the LM head with its loss.  They do what the nodes of the same name in b200moe/ops do from Python, with the same kernels in
+// Autograd nodes of the training step in C++: embedding, norm, the attention half of a block, the routed layer on one rank, the
+// LM head with its loss, routing, the gated residual norm and the linear layer in 8 bits.  They do what the nodes of the same name in b200moe/ops do from Python, with the same kernels in
 // the same order: what they save is the host's time, 20-30 us per launch and 30 per node of the backward pass (from Python's
 // second thread), which is what a small layer costs.  A step of two blocks of width 512 took 4.7 ms for 1.5 ms of kernels.
 //
 // The functions at the end answer None where an operand is not what the node takes (type, layout, alignment, device); the
 // caller then goes the general way.  Kernels come from the library that b200moe.ops.native has loaded (``bind``).
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
@@ -40,6 +42,14 @@ struct Library {
   decltype(&b2_scale_bf16) scale_bf16;
   decltype(&b2_embedding_fwd) embedding_fwd;
   decltype(&b2_embedding_bwd) embedding_bwd;
+  decltype(&b2_gemm_tn) gemm_tn;
+  decltype(&b2_route_topk) route_topk;
+  decltype(&b2_route_topk_bwd) route_topk_bwd;
+  decltype(&b2_gated_norm_fwd) gated_norm_fwd;
+  decltype(&b2_gated_norm_bwd) gated_norm_bwd;
+  decltype(&b2_gated_norm_bwd_floats) gated_norm_bwd_floats;
+  decltype(&b2_quantize_fp8) quantize_fp8;
+  decltype(&b2_gemm_fp8) gemm_fp8;
 } lib;
 
 void bind(const std::string& path) {
@@ -65,6 +75,14 @@ void bind(const std::string& path) {
   resolve(lib.scale_bf16, "b2_scale_bf16");
   resolve(lib.embedding_fwd, "b2_embedding_fwd");
   resolve(lib.embedding_bwd, "b2_embedding_bwd");
+  resolve(lib.gemm_tn, "b2_gemm_tn");
+  resolve(lib.route_topk, "b2_route_topk");
+  resolve(lib.route_topk_bwd, "b2_route_topk_bwd");
+  resolve(lib.gated_norm_fwd, "b2_gated_norm_fwd");
+  resolve(lib.gated_norm_bwd, "b2_gated_norm_bwd");
+  resolve(lib.gated_norm_bwd_floats, "b2_gated_norm_bwd_floats");
+  resolve(lib.quantize_fp8, "b2_quantize_fp8");
+  resolve(lib.gemm_fp8, "b2_gemm_fp8");
 }
 
 cudaStream_t stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
@@ -358,6 +376,150 @@ struct Head : public Function<Head> {
   }
 };
 
+// Type of the kernels that take fp32, bf16 and fp16; -1 for others.
+int float_type(const Tensor& t) {
+  return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : t.scalar_type() == at::kHalf ? 2 : -1;
+}
+// Gradients that cannot be differentiated again: where a graph of them is asked for, using it raises (as once_differentiable does for
+// the nodes in Python).
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list defined;
+  for (const Tensor& g : grads)
+    if (g.defined()) defined.push_back(g.detach().requires_grad_(true));
+  auto refuse = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked with @once_differentiable", static_cast<int64_t>(defined.size()));
+  defined = (*refuse)(std::move(defined));
+  size_t i = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = defined[i++];
+  return grads;
+}
+
+struct RouteTopk : public Function<RouteTopk> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Optional& bias, int64_t k, bool sigmoid,
+                               int64_t groups, int64_t top_groups, bool two_best, bool renormalize, double scale) {
+    const c10::cuda::CUDAGuard guard(logits.device());
+    ctx->set_materialize_grads(false);
+    const int64_t T = logits.size(0), E = logits.size(1);
+    Tensor weights = fp32({T, k}, logits), idx = at::empty({T, k}, logits.options().dtype(at::kLong));
+    check(lib.route_topk(ptr(logits), ptr(bias ? *bias : Tensor()), mut(weights), mut(idx), T, E, k, float_type(logits), sigmoid,
+                         groups, top_groups, two_best, renormalize, scale, stream()), "b2_route_topk", 1);
+    ctx->mark_non_differentiable({idx});
+    ctx->save_for_backward({logits, weights, idx});
+    ctx->saved_data["how"] = int64_t{sigmoid} + 2 * renormalize;
+    ctx->saved_data["scale"] = scale;
+    return {weights, idx};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(9);
+    if (!grads[0].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &weights = saved[1], &idx = saved[2], dweights = grads[0].contiguous();
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const int64_t how = ctx->saved_data["how"].toInt();
+    out[0] = at::empty_like(logits);
+    check(lib.route_topk_bwd(ptr(logits), ptr(weights), ptr(idx), ptr(dweights), mut(out[0]), logits.size(0), logits.size(1),
+                             idx.size(1), float_type(logits), how & 1, how >> 1, ctx->saved_data["scale"].toDouble(), stream()),
+          "b2_route_topk_bwd", 1);
+    return once(std::move(out));
+  }
+};
+
+struct GatedNorm : public Function<GatedNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& delta, const Tensor& wd, const Tensor& w,
+                               const Optional& gate, int64_t kind, int64_t seq, double scale, double eps, const Tensor& status) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    ctx->set_materialize_grads(false);
+    const int64_t D = x.size(-1), rows = x.numel() / D;
+    Tensor summed = at::empty_like(x), normed = at::empty_like(x), stats = fp32({2 * rows}, x);
+    float* const rstd = mut(stats);
+    check(lib.gated_norm_fwd(ptr(x), ptr(delta), ptr(wd), ptr(w), ptr(gate ? *gate : Tensor()), mut(summed), mut(normed), rstd,
+                             rstd + rows, rows, D, seq, float_type(x), kind, gate && gate->scalar_type() == at::kFloat, scale, eps,
+                             mut(status), stream()), "b2_gated_norm_fwd", 1);
+    ctx->save_for_backward({x, delta, wd, w, gate ? *gate : Tensor(), stats});
+    keep(ctx, {status});
+    ctx->saved_data["kind"] = kind;
+    ctx->saved_data["seq"] = seq;
+    ctx->saved_data["scale"] = scale;
+    return {summed, normed};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(10);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &delta = saved[1], &wd = saved[2], &w = saved[3], &gate = saved[4], &stats = saved[5];
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t D = x.size(-1), rows = x.numel() / D, kind = ctx->saved_data["kind"].toInt(), seq = ctx->saved_data["seq"].toInt();
+    const Tensor ds = grads[0].defined() ? grads[0].contiguous() : Tensor(), dy = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor status = kept(ctx)[0];
+    Tensor dx = at::empty_like(x), ddelta = at::empty_like(x), dwd = fp32({D}, x), dw = fp32({D}, x), dgate;
+    if (gate.defined()) dgate = at::empty_like(gate);
+    const Tensor partial = fp32({lib.gated_norm_bwd_floats(rows, D, seq, kind)}, x);
+    const float* const rstd = ptr(stats);
+    check(lib.gated_norm_bwd(ptr(ds), ptr(dy), ptr(x), ptr(delta), ptr(wd), ptr(w), ptr(gate), rstd, rstd + rows, mut(dx),
+                             mut(ddelta), mut(dwd), mut(dw), mut(dgate), mut(partial), rows, D, seq, float_type(x), kind,
+                             gate.defined() && gate.scalar_type() == at::kFloat, ctx->saved_data["scale"].toDouble(), mut(status),
+                             stream()), "b2_gated_norm_bwd", 2);
+    out[0] = dx, out[1] = ddelta, out[2] = dwd, out[3] = dw, out[4] = dgate;
+    return once(std::move(out));
+  }
+};
+
+// e4m3 values by rows of 128 and their scales, in scratch memory of the call.
+struct Rows8 {
+  Rows8(const Tensor& x, int64_t rows, int64_t cols)
+      : rows(rows), cols(cols), pitch((cols + 15) / 16 * 16), held(x, {rows * pitch, 4 * rows * ((cols + 127) / 128)}) {
+    check(lib.quantize_fp8(ptr(x), float_type(x), held[0], held[1], rows, cols, cols, pitch, rows, 1, stream()), "b2_quantize_fp8", 1);
+  }
+  // times w [N, K] transposed, or (nn) times w [K, N]
+  void times(const Tensor& w, const Tensor& scales, bool nn, const Tensor& out, const Tensor& status) const {
+    check(lib.gemm_fp8(held[0], held[1], ptr(w), ptr(scales), mut(out), rows, nn ? w.size(1) : w.size(0), cols, pitch, w.stride(0), 1,
+                       rows, scales.stride(nn), scales.stride(!nn), nn, mut(status), stream()), "b2_gemm_fp8", 1);
+  }
+  int64_t rows, cols, pitch;
+  Scratch held;
+};
+
+struct LinearFp8 : public Function<LinearFp8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& values, const Tensor& scales,
+                        const Tensor& status) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t K = weight.size(1), N = weight.size(0), rows = x.numel() / K;
+    std::vector<int64_t> sizes = x.sizes().vec();
+    sizes.back() = N;
+    Tensor y = bf16(sizes, x);
+    Rows8(x, rows, K).times(values, scales, false, y, status);
+    ctx->save_for_backward({x, values, scales});
+    keep(ctx, {weight, status});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &values = saved[1], &scales = saved[2], dy = grads[0].contiguous();
+    const std::vector<Tensor> w = kept(ctx);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t K = w[0].size(1), N = w[0].size(0), rows = x.numel() / K;
+    TORCH_CHECK(dy.scalar_type() == at::kBFloat16, "expected bfloat16, got ", dy.scalar_type());
+    const Tensor dy16 = aligned(dy) ? dy : dy.clone();
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) {
+      dx = at::empty_like(x);
+      Rows8(dy16, rows, N).times(values, scales, true, dx, w[1]);
+    }
+    const Tensor buffer = Gradient::of(w, 1)[0];
+    if (buffer.defined() || w[0].requires_grad()) {
+      const bool direct = buffer.defined() && plain(buffer, at::kFloat, x) && buffer.sizes() == w[0].sizes();
+      Tensor sum = direct ? buffer : at::empty(w[0].sizes(), w[0].options().requires_grad(false).dtype(buffer.defined() ? at::kFloat : w[0].scalar_type()));
+      check(lib.gemm_tn(ptr(dy16), ptr(x), mut(sum), nullptr, 0, N, K, rows, N, K, K, 1, nullptr, nullptr,
+                        sum.scalar_type() == at::kFloat ? 1 : 2, direct ? 1.f : 0.f, nullptr, mut(w[1]), stream()), "b2_gemm_tn", 1);
+      if (!buffer.defined()) dw = sum;
+      else if (!direct) buffer.add_(sum);
+    }
+    return once({dx, dw, Tensor(), Tensor(), Tensor()});
+  }
+};
+
 // ------------------------------------------------------------------ entry points
 Optional embedding(const Tensor& ids, const Tensor& table, const Tensor& grad) {
   if (!(ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() > 0 && ids.numel() < INT_MAX && table.dim() == 2 &&
@@ -422,6 +584,86 @@ Optional head(const Tensor& hidden, const Tensor& weight, const Tensor& targets,
   return Head::apply(hidden, weight, targets, grad, scale, chunk, status);
 }
 
+// ``score``: 0 softmax, 1 sigmoid, -1 what the caller refuses.
+std::optional<variable_list> route_topk(const Tensor& logits, const Optional& bias, int64_t k, int64_t score, int64_t groups,
+                                        int64_t top_groups, int64_t group_score, bool renormalize, double scale) {
+  if (!(logits.is_cuda() && logits.dim() == 2 && logits.size(0) > 0 && float_type(logits) >= 0 && logits.is_contiguous() && score >= 0))
+    return std::nullopt;
+  const int64_t E = logits.size(1);
+  if (!(E >= 1 && E <= 1024 && groups >= 1 && groups <= 32 && E % groups == 0 && top_groups >= 1 && top_groups <= groups && k >= 1 &&
+        k <= 32 && k <= E / groups * top_groups && (group_score == 1 || (group_score == 2 && E / groups >= 2)) && std::isfinite(scale) &&
+        scale != 0.0))
+    return std::nullopt;
+  if (bias && !(bias->dim() == 1 && bias->size(0) == E && bias->scalar_type() == at::kFloat && bias->is_contiguous() &&
+                bias->device() == logits.device() && !bias->requires_grad()))
+    return std::nullopt;
+  return RouteTopk::apply(logits, bias, k, score == 1, groups, top_groups, group_score == 2, renormalize, scale);
+}
+
+std::optional<variable_list> gated_norm(const Tensor& x, const Tensor& delta, const Tensor& wd, const Tensor& w, const Optional& gate,
+                                        double scale, double eps, const Tensor& status) {
+  const int64_t dims = x.dim();
+  if (!(x.is_cuda() && dims >= 1 && x.numel() > 0 && float_type(x) >= 0 && x.is_contiguous() && delta.sizes() == x.sizes() &&
+        delta.scalar_type() == x.scalar_type() && delta.is_contiguous() && delta.device() == x.device() && std::isfinite(scale) && eps > 0))
+    return std::nullopt;
+  const int64_t D = x.size(-1);
+  if (!(D <= 8192 && x.numel() / D < INT_MAX)) return std::nullopt;
+  for (const Tensor& t : {wd, w})
+    if (!(t.dim() == 1 && t.size(0) == D && t.scalar_type() == at::kFloat && t.is_contiguous() && t.device() == x.device()))
+      return std::nullopt;
+  int64_t kind = 0, seq = 1;                       // as _gate_kind in dense.py
+  if (gate) {
+    if (!((gate->scalar_type() == x.scalar_type() || gate->scalar_type() == at::kFloat) && gate->is_contiguous() &&
+          gate->device() == x.device()))
+      return std::nullopt;
+    std::vector<int64_t> token = x.sizes().vec(), sequence(dims, 1);
+    token.back() = 1;
+    sequence[0] = x.size(0);
+    sequence.back() = D;
+    if (gate->sizes() == x.sizes()) kind = 4;
+    else if (gate->dim() == 1 && gate->size(0) == D) kind = 1;
+    else if (gate->sizes() == at::IntArrayRef(token)) kind = 3;
+    else if (dims >= 3 && gate->sizes() == at::IntArrayRef(sequence)) kind = 2, seq = x.numel() / (x.size(0) * D);
+    else return std::nullopt;
+  }
+  return GatedNorm::apply(x, delta, wd, w, gate, kind, seq, scale, eps, status);
+}
+
+// Operands of a product that a tensor map takes: e4m3 rows of unit stride that start at multiples of 16 bytes, with fp32 scales.
+bool rows8(const Tensor& t, const Tensor& scales, int64_t block_rows, const Tensor& beside) {
+  return t.dim() == 2 && t.scalar_type() == at::kFloat8_e4m3fn && t.device() == beside.device() && t.size(0) > 0 && t.size(1) > 0 &&
+         t.stride(1) == 1 && t.stride(0) % 16 == 0 && t.stride(0) >= t.size(1) && aligned(t) && scales.dim() == 2 &&
+         scales.scalar_type() == at::kFloat && scales.device() == beside.device() &&
+         scales.size(0) == (t.size(0) + block_rows - 1) / block_rows && scales.size(1) == (t.size(1) + 127) / 128;
+}
+
+Optional matmul_fp8(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, const Tensor& status) {
+  if (!(a.is_cuda() && rows8(a, sa, 1, a) && rows8(b, sb, 128, a) && a.size(1) == b.size(1) && a.size(0) < INT_MAX)) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(a.device());
+  Tensor out = bf16({a.size(0), b.size(0)}, a);
+  check(lib.gemm_fp8(ptr(a), ptr(sa), ptr(b), ptr(sb), mut(out), a.size(0), b.size(0), a.size(1), a.stride(0), b.stride(0),
+                     sa.stride(0), sa.stride(1), sb.stride(0), sb.stride(1), 0, mut(status), stream()), "b2_gemm_fp8", 1);
+  return out;
+}
+
+Optional linear_fp8(const Tensor& x, const Tensor& weight, const Optional& values, const Optional& scales, const Tensor& status) {
+  if (!(x.is_cuda() && x.dim() >= 1 && x.numel() > 0 && plain(x, at::kBFloat16, x) && weight.dim() == 2 && weight.size(0) > 0 &&
+        x.size(-1) == weight.size(1) && weight.device() == x.device() && x.numel() / x.size(-1) < INT_MAX))
+    return std::nullopt;
+  const int64_t N = weight.size(0), K = weight.size(1);
+  if (N % 8 || K % 32 || !(weight.scalar_type() == at::kBFloat16 || weight.scalar_type() == at::kFloat)) return std::nullopt;
+  if (values) {
+    if (!(scales && rows8(*values, *scales, 128, x) && values->sizes() == weight.sizes())) return std::nullopt;
+    return LinearFp8::apply(x, weight, *values, *scales, status);
+  }
+  if (!weight.is_contiguous()) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Tensor q = at::empty({N, K}, weight.options().dtype(at::kFloat8_e4m3fn).requires_grad(false));      // K is a multiple of 16
+  const Tensor s = at::empty({(N + 127) / 128, (K + 127) / 128}, weight.options().dtype(at::kFloat).requires_grad(false));
+  check(lib.quantize_fp8(ptr(weight), float_type(weight), mut(q), mut(s), N, K, K, K, N, 128, stream()), "b2_quantize_fp8", 1);
+  return LinearFp8::apply(x, weight, q, s, status);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -434,4 +676,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_half", &attn_half, Release());
   m.def("moe_layer", &moe_layer, Release());
   m.def("head", &head, Release());
+  m.def("route_topk", &route_topk, Release());
+  m.def("gated_norm", &gated_norm, Release());
+  m.def("matmul_fp8", &matmul_fp8, Release());
+  m.def("linear_fp8", &linear_fp8, Release());
 }

@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include "chain.cuh"
+#include "entries.h"
 
 namespace b2 {
 

@@ -286,6 +286,12 @@ def gated_add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, delta_weight: torch.
 
     ``x`` and ``delta`` ``[..., D]`` have one type (bf16, fp16 or fp32; D up to 8192).  ``gate``, of that type or fp32, has
     the shape ``[D]``, ``[B, 1, D]`` for ``x [B, S, D]``, ``[..., 1]`` or that of ``x``."""
+    if use_native(x, "gated_norm"):
+        nodes = cpp_nodes(x, delta, delta_weight, weight, *(() if gate is None else (gate,)))
+        out = nodes.gated_norm(x, delta, delta_weight, weight, gate, residual_scale, eps, native.status_word(x.device)) \
+            if nodes else None
+        if out is not None:
+            return tuple(out)
     if x.shape != delta.shape or x.dim() < 1:
         raise ValueError(f"x {list(x.shape)} and delta {list(delta.shape)} must have one shape [..., D]")
     width = x.shape[-1]

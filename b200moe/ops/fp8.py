@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import backward_follows, functional as Fn, native, use_native
+from . import backward_follows, cpp_nodes, functional as Fn, native, use_native
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
@@ -47,6 +47,11 @@ def _rows_aligned(name: str, values) -> None:
 def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor) -> torch.Tensor:
     """``a [M, K] @ b [N, K]ᵀ`` as bf16 ``[M, N]``: e4m3 values, ``a_scales [M, ceil(K / 128)]``, ``b_scales [ceil(N / 128),
     ceil(K / 128)]`` (any strides).  Sums are held in fp32.  It has no gradient of its own; ``linear_fp8`` has."""
+    if use_native(a, "fp8"):
+        nodes = cpp_nodes(a, a_scales, b, b_scales)
+        out = nodes.matmul_fp8(a, a_scales, b, b_scales, native.status_word(a.device)) if nodes else None
+        if out is not None:
+            return out
     _check_operand("a", a, a_scales, 1)
     _check_operand("b", b, b_scales, 128)
     if a.shape[1] != b.shape[1] or a.device != b.device:
@@ -112,6 +117,12 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_fp8=None) -> torch.
     when the weight changes).  The gradient of ``x`` is the same kind of product of ``dy``, quantised by rows of 128, with the
     same values of the weight; that of the weight is the bf16 product ``dyᵀ x``, added to ``weight.main_grad`` where there is
     one, like ``linear``'s."""
+    if use_native(x, "fp8") and getattr(weight, "pending_gather", None) is None:
+        values, scales = (None, None) if weight_fp8 is None else weight_fp8
+        nodes = cpp_nodes(x, weight, *(() if values is None else (values, scales)))
+        out = nodes.linear_fp8(x, weight, values, scales, native.status_word(x.device)) if nodes else None
+        if out is not None:
+            return out
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x {list(x.shape)} and weight {list(weight.shape)} must share their last dimension")
     if x.device != weight.device:

@@ -26,7 +26,7 @@ import torch.distributed as dist
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from . import backward_follows, functional as Fn, native, use_native
+from . import backward_follows, cpp_nodes, functional as Fn, native, use_native
 
 ALIGN = 128
 
@@ -52,6 +52,9 @@ def router_top2(logits: torch.Tensor):
     if use_native(logits, "router"):
         return _RouterTop2.apply(logits)
     return Fn.router_top2_ref(logits, 2)
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
 
 
 class _RouteTopk(torch.autograd.Function):
@@ -84,13 +87,19 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: to
     Experts come best first, the lower index first where two are equal; without a bias they are compared by their logits.  The
     choice is that of exact arithmetic: scores that are too close for fp32 are compared in fp64.  A logit of -inf (or NaN)
     masks an expert: it comes after all others of the chosen groups, with weight 0; +inf counts as the largest number."""
+    if use_native(logits, "route"):
+        nodes = cpp_nodes(logits) if bias is None else cpp_nodes(logits, bias)
+        out = nodes.route_topk(logits, bias, k, _SCORES.get(score, -1), groups, groups if top_groups is None else top_groups,
+                               group_score, renormalize, scale) if nodes else None
+        if out is not None:
+            return tuple(out)
     if logits.dim() != 2:
         raise ValueError(f"logits must be [tokens, experts], got {tuple(logits.shape)}")
     if not logits.dtype.is_floating_point:
         raise TypeError(f"logits must be floating point, got {logits.dtype}")
     experts = logits.shape[1]
     top_groups = groups if top_groups is None else top_groups
-    if score not in ("softmax", "sigmoid"):
+    if score not in _SCORES:
         raise ValueError(f"score must be softmax or sigmoid, got {score!r}")
     if not (1 <= groups <= 32 and experts >= 1 and experts % groups == 0 and 1 <= top_groups <= groups):
         raise ValueError(f"{experts} experts cannot form {groups} groups of which {top_groups} stay (at most 32 groups)")

@@ -462,3 +462,95 @@ def test_a_block_of_all_operators_forward_and_backward():
             leaf.add_(step * direction)
         slope = float((grad.double() * direction.double()).sum())
         assert abs((high - low) / (2 * step) - slope) < 0.05 * abs(slope), (high, low, slope)
+
+
+@pytest.fixture
+def in_python(monkeypatch):
+    """Runs a function with the nodes in Python, which also take what the C++ nodes leave to them."""
+    from b200moe.ops import dense, fp8, moe
+
+    def run(f):
+        with monkeypatch.context() as m:
+            for module in (dense, fp8, moe):
+                m.setattr(module, "cpp_nodes", lambda *_: None)
+            return f()
+    return run
+
+
+def _same(a, b):
+    assert len(a) == len(b) and all(x.dtype == y.dtype and torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_cpp_nodes_do_what_the_python_nodes_do(in_python):
+    from b200moe.ops import native
+    assert native.nodes() is not None
+    logits = torch.randn(130, 96, device="cuda").bfloat16().requires_grad_()
+    bias, g = torch.randn(96, device="cuda") * 0.1, torch.randn(130, 5, device="cuda")
+    for how in (dict(score="sigmoid", bias=bias, groups=8, top_groups=3, group_score=2, scale=2.5), dict(renormalize=False), dict()):
+        def route():
+            weights, idx = ops.route_topk(logits, 5, **how)
+            return [weights.detach(), idx, *torch.autograd.grad(weights, logits, g)]
+        before = native.nodes().launches()
+        _same(route(), in_python(route))
+        assert native.nodes().launches() == before + 2
+    for kind in ("none", "channel", "sequence", "token", "full"):
+        x, delta, wd, w, gate = _norm_case(3, 41, 264, kind, torch.bfloat16, torch.float32)
+        leaves = [t.requires_grad_() for t in (x, delta, wd, w) + (() if gate is None else (gate,))]
+        ds, dy = torch.randn_like(x), torch.randn_like(x)
+        for use in ((0, 1), (0,), (1,)):
+            def norm():
+                out = ops.gated_add_rmsnorm(*leaves[:4], gate=gate, residual_scale=0.8)
+                return [t.detach() for t in out] + list(torch.autograd.grad([out[i] for i in use], leaves, [(ds, dy)[i] for i in use]))
+            before = native.nodes().launches()
+            _same(norm(), in_python(norm))
+            assert native.nodes().launches() == before + 3
+    x = torch.randn(2, 65, 160, device="cuda").bfloat16().requires_grad_()
+    dy = torch.randn(2, 65, 264, device="cuda").bfloat16()
+    for dtype in (torch.bfloat16, torch.float32):
+        weight = (torch.randn(264, 160, device="cuda") * 0.1).to(dtype).requires_grad_()
+        for packed in (None, ops.quantize_fp8(weight, 128)):
+            def linear():
+                y = ops.linear_fp8(x, weight, weight_fp8=packed)
+                return [y.detach(), *torch.autograd.grad(y, (x, weight), dy)]
+            before = native.nodes().launches()
+            _same(linear(), in_python(linear))
+            assert native.nodes().launches() > before
+    weight.main_grad = torch.ones_like(weight)
+    torch.autograd.backward(ops.linear_fp8(x, weight), dy)
+    first = weight.main_grad.clone()
+    weight.main_grad.fill_(1)
+    in_python(lambda: torch.autograd.backward(ops.linear_fp8(x, weight), dy))
+    assert torch.equal(first, weight.main_grad) and weight.grad is None
+    a, sa = _operand(33, 160, 1)
+    b, sb = _operand(50, 160, 128)
+    _same([ops.matmul_fp8(a, sa, b, sb)], [in_python(lambda: ops.matmul_fp8(a, sa, b, sb))])
+
+
+def test_gradients_are_not_differentiated_twice(in_python):
+    logits = torch.randn(9, 16, device="cuda", requires_grad=True)
+    x = torch.randn(4, 64, device="cuda").bfloat16().requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    weight = torch.randn(32, 64, device="cuda").bfloat16().requires_grad_()
+    for f in (lambda: (ops.route_topk(logits, 3)[0], logits), lambda: (ops.gated_add_rmsnorm(x, x, w, w)[1], w),
+              lambda: (ops.linear_fp8(x, weight), x)):
+        for run in (lambda f: f(), in_python):
+            out, leaf = run(f)
+            (grad,) = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                grad.float().sum().backward()
+
+
+def test_refusals_reach_the_caller_through_the_nodes():
+    x = torch.zeros(4, 12, device="cuda")
+    for bad in (dict(k=0), dict(k=13), dict(k=2, score="relu"), dict(k=2, groups=5), dict(k=7, groups=4, top_groups=2),
+                dict(k=2, scale=0.0), dict(k=2, bias=torch.zeros(11, device="cuda")), dict(k=2, bias=torch.zeros(12))):
+        with pytest.raises(ValueError):
+            ops.route_topk(x, **bad)
+    with pytest.raises(TypeError):
+        ops.route_topk(x.double(), 2)
+    w = torch.ones(12, device="cuda")
+    for bad in (dict(gate=torch.ones(11, device="cuda")), dict(eps=0.0), dict(residual_scale=math.inf), dict(gate=torch.ones(12))):
+        with pytest.raises(ValueError):
+            ops.gated_add_rmsnorm(x, x, w, w, **bad)
+    with pytest.raises(TypeError):
+        ops.gated_add_rmsnorm(x.double(), x.double(), w, w)

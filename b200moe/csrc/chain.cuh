@@ -7,6 +7,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <utility>
 
 namespace b2 {
@@ -30,6 +31,18 @@ static inline cudaError_t launch_next(void (*kernel)(Params...), dim3 grid, dim3
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Lets a kernel have more than 48 KiB of dynamic shared memory on the current device; the runtime is asked once per kernel and device.
+template <auto KERNEL>
+static inline cudaError_t allow_shared(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int device = 0;
+  cudaError_t r = cudaGetDevice(&device);
+  if (r != cudaSuccess || (device < 64 && (done.load(std::memory_order_relaxed) >> device & 1))) return r;
+  r = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (r == cudaSuccess && device < 64) done.fetch_or(1ull << device, std::memory_order_relaxed);
+  return r;
 }
 
 }  // namespace b2

@@ -27,7 +27,7 @@
 namespace b2 {
 
 constexpr float E4M3_MAX = 448.f;
-constexpr float SMALLEST_SCALE = 7.52316384526264e-37f;     // 2^-120
+constexpr float SMALLEST_SCALE = 0x1p-120f;
 constexpr int F8_BM = 128, F8_BK = 128;
 constexpr int F8_EPI_WARPS = 8, F8_THREADS = 128 + 32 * F8_EPI_WARPS;
 // Registers: 384 threads x 168 at launch = 128 x 72 + 256 x 216 afterwards.
@@ -155,36 +155,36 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
   }
 }
 
-// One scale for 128 x 128 values: a CTA per block, 64 values a thread.
+// One scale for 128 x 128 values: a CTA per block, 32 values a thread, so that enough threads fit for their loads to fill the memory.
 template <typename T>
-__global__ void __launch_bounds__(256, 3) quantize_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
-                                                              float* __restrict__ scales, int M, int K, long long ldx,
-                                                              long long pitch, int aligned) {
+__global__ void __launch_bounds__(512, 3) quantize_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                                 float* __restrict__ scales, int M, int K, long long ldx,
+                                                                 long long pitch, int aligned) {
   chain_begin();
-  __shared__ float most[8];
+  __shared__ float most[16];
   const int kb = blockIdx.x, lane16 = threadIdx.x & 15, col = kb * 128 + lane16 * 8;
   for (long long mb = blockIdx.y; mb * 128 < M; mb += gridDim.y) {
     const long long row0 = mb * 128 + (threadIdx.x >> 4);
-    Values8<T> f[8];
+    Values8<T> f[4];
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const long long row = row0 + i * 16;
+    for (int i = 0; i < 4; ++i) {
+      const long long row = row0 + i * 32;
       f[i].load(x + row * ldx + col, row < M ? K - col : 0, aligned);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, largest8(f[i]));
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, largest8(f[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     __syncthreads();
     if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, most[i]);
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, most[i]);
     const BlockScale s = block_scale(m);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const long long row = row0 + i * 16;
+    for (int i = 0; i < 4; ++i) {
+      const long long row = row0 + i * 32;
       if (row < M && col < pitch) store8(q + row * pitch + col, s, f[i]);
     }
     if (threadIdx.x == 0) scales[mb * gridDim.x + kb] = s.scale;
@@ -512,12 +512,8 @@ static int f8_sms() {
 
 template <int BN, int B_MN, int SPLIT>
 static int launch_fp8(const Fp8Params& p, cudaStream_t s) {
-  auto kernel = gemm_fp8_kernel<BN, B_MN, SPLIT>;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F8Cfg<BN>::SMEM) != cudaSuccess) return -3;
-    set = true;
-  }
+  constexpr auto kernel = gemm_fp8_kernel<BN, B_MN, SPLIT>;
+  if (allow_shared<kernel>(F8Cfg<BN>::SMEM) != cudaSuccess) return -3;
   const long long tiles = static_cast<long long>((p.M + F8_BM - 1) / F8_BM) * ((p.N + BN - 1) / BN);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -588,7 +584,7 @@ static cudaError_t launch_quantize(const void* x, void* q, float* scales, int M,
   if (block_rows == 128) {
     const long long rows = (M + 127) / 128;
     return launch_next(quantize_blocks_kernel<T>, dim3(static_cast<unsigned>(across), static_cast<unsigned>(rows < 32768 ? rows : 32768)),
-                       256, 0, s, in, out, scales, M, K, ldx, pitch, aligned);
+                       512, 0, s, in, out, scales, M, K, ldx, pitch, aligned);
   }
   // few blocks are spread over more CTAs
   if (blocks <= f8_sms() * 64LL)

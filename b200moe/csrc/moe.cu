@@ -454,13 +454,7 @@ int b2_moe_plan(const long long* idx, int slots, int E, int* slot_row, int* row_
                 int* meta, int* counts, int capacity_rows, cudaStream_t s) {
   if (E < 1) return -10;
   if (E > 1024) return -11;                 // 144 bytes of shared memory an expert
-  if (E > 300) {
-    static bool set = false;
-    if (!set) {
-      if (cudaFuncSetAttribute(moe_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess) return -3;
-      set = true;
-    }
-  }
+  if (E > 300 && allow_shared<moe_plan_kernel>(160 * 1024) != cudaSuccess) return -3;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -9,6 +9,8 @@
 // own keys (a network of minima and maxima, no indices), then k steps take the best of the lanes' first keys and remove it; the
 // index of a chosen key is looked up afterwards among the lane's keys, for all chosen ones at once.
 //
+// Bound by integer minima, comparisons and selections, which the ALU issues every other cycle, beyond 100 experts.
+//
 // The choice is that of exact arithmetic.  Comparisons of logits are exact as they are.  Comparisons of scores (a bias, a
 // sum of two) are made in fp32 with the fast exponential and division first, and those that decided something are checked
 // against a bound on the error of both sides; a row in which one is closer than that is worked out again in 64 bits, by a whole
@@ -38,6 +40,8 @@ struct RouteParams {
   long long T;
   int E, k, type, sigmoid, groups, top_groups, two_best, renormalize;
   float scale;
+  int size;                  // experts of a group
+  int lane_shift;            // GROUPS_ALIGNED: a group is 2^lane_shift lanes
 };
 
 // NaN counts as masked (a maximum leaves it out), infinity as the largest number.
@@ -261,7 +265,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, long long row, const
   }
   close = false;
   unsigned allowed = ALL;                          // one bit per group
-  const int size = MODE == GROUPS_NONE ? p.E : p.E / p.groups;
+  const int size = p.size;
   if (MODE != GROUPS_NONE) {
     float best = -INFINITY, second = -INFINITY;
     if (MODE == GROUPS_ALIGNED) {                  // a group is a run of 2^n whole lanes
@@ -270,14 +274,13 @@ __device__ __forceinline__ int choose(const RouteParams& p, long long row, const
         second = fmaxf(second, fminf(best, key[j]));
         best = fmaxf(best, key[j]);
       }
-      const int lanes = size / V;
-      for (int o = 1; o < lanes; o <<= 1) {
+      for (int o = 1; o < 1 << p.lane_shift; o <<= 1) {
         const float b = __shfl_xor_sync(ALL, best, o), s = __shfl_xor_sync(ALL, second, o);
         second = fmaxf(fminf(best, b), fmaxf(second, s));
         best = fmaxf(best, b);
       }
-      best = __shfl_sync(ALL, best, min(lane * lanes, LANES - 1), LANES);
-      second = __shfl_sync(ALL, second, min(lane * lanes, LANES - 1), LANES);
+      best = __shfl_sync(ALL, best, min(lane << p.lane_shift, LANES - 1), LANES);
+      second = __shfl_sync(ALL, second, min(lane << p.lane_shift, LANES - 1), LANES);
     } else {                                       // through shared memory, a lane per group
 #pragma unroll
       for (int j = 0; j < V; ++j)
@@ -315,7 +318,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, long long row, const
   }
   // Without a bias experts are compared by their logits, whatever the groups were compared by.
   uint32_t h[V];
-  const bool lane_here = MODE != GROUPS_ALIGNED || (first < p.E && (allowed >> min(first / size, 31) & 1));
+  const bool lane_here = MODE != GROUPS_ALIGNED || (first < p.E && (allowed >> (lane >> p.lane_shift) & 1));
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const bool here = MODE == GROUPS_ALIGNED ? lane_here
@@ -546,9 +549,9 @@ __global__ void __launch_bounds__(route_warps(V) * 32, 4) route_fwd_kernel(const
     // softmax: the other experts cancel.  Sigmoids below -60 are exp(x) to the last bit, and their sum could vanish.
     const float top = row_max_f<LANES>(xe);
     if (!p.sigmoid || top < -60.f) w = xe == -INFINITY ? 0.f : expf(xe - top);
-    else w = xe == -INFINITY ? 0.f : 1.f / (1.f + expf(-xe));
+    else w = xe == -INFINITY ? 0.f : __fdividef(1.f, 1.f + expf(-xe));       // 2 units in the last place
     const float total = row_add<LANES>(w);
-    w = total == 0.f ? 0.f : w / total;
+    w = total == 0.f ? 0.f : __fdividef(w, total);
   } else {
     RowStats st = {0.f, 1.f};
     if (!p.sigmoid) st = softmax_stats<LANES, false, V>(x);
@@ -645,12 +648,11 @@ __global__ void __launch_bounds__(route_warps(V) * 32) route_bwd_kernel(const Ro
 
 // Whether a group is a run of 2^n lanes of V logits.
 static bool whole_lanes(const RouteParams& p, int V) {
-  const int size = p.E / p.groups;
-  return size % V == 0 && ((size / V) & (size / V - 1)) == 0;
+  return p.size % V == 0 && ((p.size / V) & (p.size / V - 1)) == 0;
 }
 
 template <int LANES, int V>
-static int launch_route(const RouteParams& p, cudaStream_t s) {
+static int launch_route(RouteParams p, cudaStream_t s) {
   constexpr int WARPS = route_warps(V);
   const long long grid = (p.T + WARPS * (32 / LANES) - 1) / (WARPS * (32 / LANES));
   if (grid > 0x7fffffffLL) return -12;
@@ -659,6 +661,7 @@ static int launch_route(const RouteParams& p, cudaStream_t s) {
   if (p.top_groups == p.groups) {
     r = launch_next(route_fwd_kernel<LANES, V, GROUPS_NONE>, ctas, WARPS * 32, 0, s, p);
   } else if constexpr (LANES == 32) {
+    for (int lanes = p.size / V; lanes > 1; lanes >>= 1) ++p.lane_shift;
     if (whole_lanes(p, V)) r = launch_next(route_fwd_kernel<32, V, GROUPS_ALIGNED>, ctas, WARPS * 32, 0, s, p);
     else r = launch_next(route_fwd_kernel<32, V, GROUPS_ANY>, ctas, WARPS * 32, 0, s, p);
   }
@@ -722,7 +725,8 @@ extern "C" {
 // logits [T, E] contiguous (type 0 fp32, 1 bf16, 2 fp16), bias fp32 [E] or null -> weights fp32 [T, k], idx int64 [T, k].
 int b2_route_topk(const void* logits, const float* bias, float* weights, long long* idx, long long T, int E, int k, int type,
                   int sigmoid, int groups, int top_groups, int two_best, int renormalize, float scale, cudaStream_t s) {
-  const RouteParams p = {logits, bias, weights, idx, T, E, k, type, sigmoid, groups, top_groups, two_best, renormalize, scale};
+  const RouteParams p = {logits, bias, weights, idx, T, E, k, type, sigmoid, groups, top_groups, two_best, renormalize, scale,
+                         groups > 0 ? E / groups : 0, 0};
   return route(p, nullptr, nullptr, s);
 }
 
@@ -730,7 +734,7 @@ int b2_route_topk(const void* logits, const float* bias, float* weights, long lo
 int b2_route_topk_bwd(const void* logits, const float* weights, const long long* idx, const float* dweights, void* dlogits,
                       long long T, int E, int k, int type, int sigmoid, int renormalize, float scale, cudaStream_t s) {
   const RouteParams p = {logits, nullptr, const_cast<float*>(weights), const_cast<long long*>(idx), T, E, k, type, sigmoid,
-                         1, 1, 0, renormalize, scale};
+                         1, 1, 0, renormalize, scale, E, 0};
   return route(p, dweights, dlogits, s);
 }
 

@@ -99,7 +99,7 @@ class _LinearFp8(torch.autograd.Function):
         dx = _product(dy2d, values, scales, False).view(ctx.shape) if ctx.needs_input_grad[0] else None
         main_grad = getattr(weight, "main_grad", None)
         dw = None
-        on_gpu = use_native(dy2d, "gemm")
+        on_gpu = use_native(dy2d, "gemm") and dy2d.shape[0] > 0       # no rows: zeros
         if main_grad is not None:
             if on_gpu:
                 native.gemm_tn(dy2d, x2d, out=main_grad, accumulate=True)
@@ -123,8 +123,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_fp8=None) -> torch.
         out = nodes.linear_fp8(x, weight, values, scales, native.status_word(x.device)) if nodes else None
         if out is not None:
             return out
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"x {list(x.shape)} and weight {list(weight.shape)} must share their last dimension")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
+        raise ValueError(f"x {list(x.shape)} and weight {list(weight.shape)} must share their last dimension, and the weight have a row")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
     if getattr(weight, "pending_gather", None) is not None:

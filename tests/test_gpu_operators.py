@@ -376,7 +376,10 @@ def test_linear_fp8_layouts_streams_and_graphs():
         y = ops.linear_fp8(x, weight, weight_fp8=packed)
     graph.replay()
     assert torch.equal(y, want_y)
-    assert ops.linear_fp8(x[:0], weight).shape == (0, N)
+    none = x[:0].clone().requires_grad_()
+    y = ops.linear_fp8(none, weight)
+    dx, dw = torch.autograd.grad(y, (none, weight), torch.empty_like(y))
+    assert y.shape == (0, N) and dx.shape == (0, K) and dw.shape == (N, K) and not dw.any()
 
 
 def test_fp8_refuses_on_the_gpu():

@@ -4,6 +4,8 @@
 //   quantise   scale = max(largest / 448, 2^-120), value = x / scale rounded to e4m3 (448 is its largest number)
 //   product    y[m, n] = sum over blocks b of  sa[m, b] sb[n / 128, b] * (sum over the 128 k of b of a[m, k] w[n, k])
 //
+// The two scales are multiplied first: results below 2^-102, whose product of scales may be subnormal, lose bits.
+//
 // The data gradient dx = dy W takes the weight as it is stored: its rows are the reduction, so B is read along MN, and a
 // 128 x 128 block has the same scale either way.
 //
@@ -30,8 +32,8 @@ constexpr float E4M3_MAX = 448.f;
 constexpr float SMALLEST_SCALE = 0x1p-120f;
 constexpr int F8_BM = 128, F8_BK = 128;
 constexpr int F8_EPI_WARPS = 8, F8_THREADS = 128 + 32 * F8_EPI_WARPS;
-// Registers: 384 threads x 168 at launch = 128 x 72 + 256 x 216 afterwards.
-constexpr int F8_FEW = 72, F8_MANY = 216;
+// Registers: 384 threads x 168 at launch and at the end, 128 x 72 + 256 x 216 in between.
+constexpr int F8_EVEN = 168, F8_FEW = 72, F8_MANY = 216;
 constexpr int F8_GROUP_M = 8;
 constexpr int F8_AHEAD = 4;
 constexpr int F8_STAGING = F8_EPI_WARPS * 2048;
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
             if (kb0 + i >= kb_end) break;
             const float4 v = ahead[i];
             ahead[i] = fetch(kb0 + i + F8_AHEAD);
-            if (!mbar_wait(&tmem_empty[slot], slot_phase)) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[slot], slot_phase))) {       // the lanes go on together
               *abort_flag = 1;
               atomicExch(p.status, 3);
               break;
@@ -380,6 +382,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
         }
       }
     }
+    __syncwarp();
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_EVEN));      // the same for all behind the branches
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_MANY));
     // ------------------------------------------------------------ scales, sums and stores
@@ -396,7 +400,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
 #pragma unroll
       for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
       for (int kb = kb_begin; kb < kb_end; ++kb) {
-        if (!mbar_wait(&tmem_full[slot], slot_phase)) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[slot], slot_phase))) {       // the lanes go on together
           *abort_flag = 1;
           atomicExch(p.status, 4);
           break;
@@ -464,6 +468,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_fp8_kernel(const __grid_co
         __syncwarp();
       }
     }
+    __syncwarp();
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8_EVEN));
   }
   if (SPLIT) {
     __syncwarp();

@@ -397,19 +397,25 @@ variable_list once(variable_list grads) {
 }
 
 struct RouteTopk : public Function<RouteTopk> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Optional& bias, int64_t k, bool sigmoid,
-                               int64_t groups, int64_t top_groups, bool two_best, bool renormalize, double scale) {
+  // weights and idx
+  static variable_list run(const Tensor& logits, const Optional& bias, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups,
+                           bool two_best, bool renormalize, double scale) {
     const c10::cuda::CUDAGuard guard(logits.device());
-    ctx->set_materialize_grads(false);
     const int64_t T = logits.size(0), E = logits.size(1);
     Tensor weights = fp32({T, k}, logits), idx = at::empty({T, k}, logits.options().dtype(at::kLong));
     check(lib.route_topk(ptr(logits), ptr(bias ? *bias : Tensor()), mut(weights), mut(idx), T, E, k, float_type(logits), sigmoid,
                          groups, top_groups, two_best, renormalize, scale, stream()), "b2_route_topk", 1);
-    ctx->mark_non_differentiable({idx});
-    ctx->save_for_backward({logits, weights, idx});
+    return {weights, idx};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Optional& bias, int64_t k, bool sigmoid,
+                               int64_t groups, int64_t top_groups, bool two_best, bool renormalize, double scale) {
+    ctx->set_materialize_grads(false);
+    variable_list out = run(logits, bias, k, sigmoid, groups, top_groups, two_best, renormalize, scale);
+    ctx->mark_non_differentiable({out[1]});
+    ctx->save_for_backward({logits, out[0], out[1]});
     ctx->saved_data["how"] = int64_t{sigmoid} + 2 * renormalize;
     ctx->saved_data["scale"] = scale;
-    return {weights, idx};
+    return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(9);
@@ -427,22 +433,29 @@ struct RouteTopk : public Function<RouteTopk> {
 };
 
 struct GatedNorm : public Function<GatedNorm> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& delta, const Tensor& wd, const Tensor& w,
-                               const Optional& gate, int64_t kind, int64_t seq, double scale, double eps, const Tensor& status) {
+  // the sum, its norm, and 1 / rms of delta and of the sum
+  static variable_list run(const Tensor& x, const Tensor& delta, const Tensor& wd, const Tensor& w, const Optional& gate,
+                           int64_t kind, int64_t seq, double scale, double eps, const Tensor& status) {
     const c10::cuda::CUDAGuard guard(x.device());
-    ctx->set_materialize_grads(false);
     const int64_t D = x.size(-1), rows = x.numel() / D;
     Tensor summed = at::empty_like(x), normed = at::empty_like(x), stats = fp32({2 * rows}, x);
     float* const rstd = mut(stats);
     check(lib.gated_norm_fwd(ptr(x), ptr(delta), ptr(wd), ptr(w), ptr(gate ? *gate : Tensor()), mut(summed), mut(normed), rstd,
                              rstd + rows, rows, D, seq, float_type(x), kind, gate && gate->scalar_type() == at::kFloat, scale, eps,
                              mut(status), stream()), "b2_gated_norm_fwd", 1);
-    ctx->save_for_backward({x, delta, wd, w, gate ? *gate : Tensor(), stats});
+    return {summed, normed, stats};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& delta, const Tensor& wd, const Tensor& w,
+                               const Optional& gate, int64_t kind, int64_t seq, double scale, double eps, const Tensor& status) {
+    ctx->set_materialize_grads(false);
+    variable_list out = run(x, delta, wd, w, gate, kind, seq, scale, eps, status);
+    ctx->save_for_backward({x, delta, wd, w, gate ? *gate : Tensor(), out[2]});
     keep(ctx, {status});
     ctx->saved_data["kind"] = kind;
     ctx->saved_data["seq"] = seq;
     ctx->saved_data["scale"] = scale;
-    return {summed, normed};
+    out.pop_back();
+    return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(10);
@@ -482,14 +495,18 @@ struct Rows8 {
 };
 
 struct LinearFp8 : public Function<LinearFp8> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& values, const Tensor& scales,
-                        const Tensor& status) {
+  static Tensor run(const Tensor& x, const Tensor& weight, const Tensor& values, const Tensor& scales, const Tensor& status) {
     const c10::cuda::CUDAGuard guard(x.device());
     const int64_t K = weight.size(1), N = weight.size(0), rows = x.numel() / K;
     std::vector<int64_t> sizes = x.sizes().vec();
     sizes.back() = N;
     Tensor y = bf16(sizes, x);
     Rows8(x, rows, K).times(values, scales, false, y, status);
+    return y;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& values, const Tensor& scales,
+                        const Tensor& status) {
+    Tensor y = run(x, weight, values, scales, status);
     ctx->save_for_backward({x, values, scales});
     keep(ctx, {weight, status});
     return y;
@@ -597,6 +614,7 @@ std::optional<variable_list> route_topk(const Tensor& logits, const Optional& bi
   if (bias && !(bias->dim() == 1 && bias->size(0) == E && bias->scalar_type() == at::kFloat && bias->is_contiguous() &&
                 bias->device() == logits.device() && !bias->requires_grad()))
     return std::nullopt;
+  if (!follows({logits})) return RouteTopk::run(logits, bias, k, score == 1, groups, top_groups, group_score == 2, renormalize, scale);
   return RouteTopk::apply(logits, bias, k, score == 1, groups, top_groups, group_score == 2, renormalize, scale);
 }
 
@@ -626,6 +644,11 @@ std::optional<variable_list> gated_norm(const Tensor& x, const Tensor& delta, co
     else if (dims >= 3 && gate->sizes() == at::IntArrayRef(sequence)) kind = 2, seq = x.numel() / (x.size(0) * D);
     else return std::nullopt;
   }
+  if (!follows({x, delta, wd, w, gate ? *gate : Tensor()})) {
+    variable_list out = GatedNorm::run(x, delta, wd, w, gate, kind, seq, scale, eps, status);
+    out.pop_back();
+    return out;
+  }
   return GatedNorm::apply(x, delta, wd, w, gate, kind, seq, scale, eps, status);
 }
 
@@ -654,14 +677,14 @@ Optional linear_fp8(const Tensor& x, const Tensor& weight, const Optional& value
   if (N % 8 || K % 32 || !(weight.scalar_type() == at::kBFloat16 || weight.scalar_type() == at::kFloat)) return std::nullopt;
   if (values) {
     if (!(scales && rows8(*values, *scales, 128, x) && values->sizes() == weight.sizes())) return std::nullopt;
-    return LinearFp8::apply(x, weight, *values, *scales, status);
+    return follows({x, weight}) ? LinearFp8::apply(x, weight, *values, *scales, status) : LinearFp8::run(x, weight, *values, *scales, status);
   }
   if (!weight.is_contiguous()) return std::nullopt;
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor q = at::empty({N, K}, weight.options().dtype(at::kFloat8_e4m3fn).requires_grad(false));      // K is a multiple of 16
   const Tensor s = at::empty({(N + 127) / 128, (K + 127) / 128}, weight.options().dtype(at::kFloat).requires_grad(false));
   check(lib.quantize_fp8(ptr(weight), float_type(weight), mut(q), mut(s), N, K, K, K, N, 128, stream()), "b2_quantize_fp8", 1);
-  return LinearFp8::apply(x, weight, q, s, status);
+  return follows({x, weight}) ? LinearFp8::apply(x, weight, q, s, status) : LinearFp8::run(x, weight, q, s, status);
 }
 
 }  // namespace

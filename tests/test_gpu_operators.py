@@ -382,6 +382,59 @@ def test_linear_fp8_layouts_streams_and_graphs():
     assert y.shape == (0, N) and dx.shape == (0, K) and dw.shape == (N, K) and not dw.any()
 
 
+def test_linear_fp8_training_step_in_a_graph():
+    M, N, K = 130, 256, 192
+    x = torch.randn(M, K, device="cuda").bfloat16().requires_grad_()
+    weight = (torch.randn(N, K, device="cuda") * 0.1).bfloat16().requires_grad_()
+    dy = torch.randn(M, N, device="cuda").bfloat16()
+
+    def step():
+        y = ops.linear_fp8(x, weight)
+        return [y.detach(), *torch.autograd.grad(y, (x, weight), dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    captured = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            captured.append(step())
+    with torch.no_grad():
+        x.mul_(0.5)
+        dy.add_(1)
+    for graph in graphs + graphs:
+        graph.replay()
+    exact = step()
+    for results in captured:
+        assert all(torch.equal(a, b) for a, b in zip(results, exact))
+
+
+def test_products_beyond_32_bits_of_offset():
+    rows, K, N = 2 ** 19 + 130, 4128, 16
+    x = torch.zeros(rows, K, device="cuda", dtype=torch.bfloat16)
+    x[-200:] = torch.randn(200, K, device="cuda").bfloat16()
+    values, scales = ops.quantize_fp8(x)
+    v, s = want.quantize(x[-200:], 1)
+    assert torch.equal(values[-200:].double().cpu(), v) and torch.equal(scales[-200:].cpu(), s)
+    b, sb = _operand(N, K, 128)
+    y = ops.matmul_fp8(values, scales, b, sb)
+    _check_product(y[-200:], (v * want.spread(s, 200, K, 1)).cuda(), b.double() * want.spread(sb, N, K, 128))
+    assert not y[:-200].any()
+
+
+def test_linear_fp8_of_widths_that_have_no_gradient_products():
+    x, w = torch.randn(9, 1000, device="cuda").bfloat16(), (torch.randn(77, 1000, device="cuda") * 0.1).bfloat16()
+    (vx, sx), (vw, sw) = want.quantize(x, 1), want.quantize(w, 128)
+    exact = (vx * want.spread(sx, 9, 1000, 1)).cuda(), (vw * want.spread(sw, 77, 1000, 128)).cuda()
+    _check_product(ops.linear_fp8(x, w), *exact)
+    _check_product(ops.linear_fp8(x, w, weight_fp8=ops.quantize_fp8(w, 128)), *exact)
+    dx = torch.autograd.grad(ops.linear_fp8(x.requires_grad_(), w), x, torch.ones(9, 77, device="cuda").bfloat16())[0]
+    _check_product(dx, torch.ones(9, 77, device="cuda", dtype=torch.float64), exact[1].t())
+
+
 def test_fp8_refuses_on_the_gpu():
     a, sa = _operand(5, 200, 1)
     b, sb = _operand(7, 200, 128)
@@ -401,7 +454,7 @@ def test_fp8_refuses_on_the_gpu():
 
 
 # ------------------------------------------------------------------------------ together
-@pytest.mark.parametrize("T,E,k", [(1, 8, 1), (77, 8, 3), (300, 64, 8), (129, 320, 6), (1000, 16, 2)])
+@pytest.mark.parametrize("T,E,k", [(1, 8, 1), (77, 8, 3), (300, 64, 8), (129, 320, 6), (1000, 16, 2), (40, 1024, 32)])
 def test_moe_ffn_for_any_number_of_experts_per_token(T, E, k):
     D, F = 128, 256
     x = torch.randn(T, D, device="cuda").bfloat16().requires_grad_()

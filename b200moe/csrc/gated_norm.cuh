@@ -51,7 +51,7 @@ struct GatedNormParams {
   void* dgate;               // [rows] or [rows, D] (GATE_TOKEN, GATE_FULL)
   float* partial;            // [2][CTAs][D] column sums, then for GATE_SEQUENCE [CTAs + sequences][rows at a time][D]
   int* status;               // device word, non-zero: a wait ran out
-  int rows, D, seq, gate_kind, gate_f32, aligned, stages;
+  int rows, D, seq, gate_kind, gate_f32, aligned, stages, ctas_per_sm;
   float residual_scale, eps;
 };
 
@@ -252,8 +252,6 @@ __device__ __forceinline__ void load_gwd(const GatedNormParams& p, long long row
   }
 }
 
-template <int W> constexpr int gn_ctas_per_sm() { return W == 16 ? 1 : 2; }
-
 // ------------------------------------------------------------------ host side
 static int gn_sms() {
   static int sms = 0;
@@ -285,8 +283,8 @@ static uint32_t gn_extra_bytes(const GatedNormParams& p, bool backward) {
   // backward: w, and dw_d of a gate per sequence
   return backward ? (gn_width(p.D) == 16 ? 512 : 256) * GN_VECS * 8 * 4 * (p.gate_kind == GATE_SEQUENCE ? 2 : 1) : 0;
 }
-static int gn_stages(const GatedNormParams& p, int type, bool backward) {
-  const uint32_t per_cta = (gn_width(p.D) == 16 ? 226 : 113) * 1024u - 600u - gn_extra_bytes(p, backward);
+static int gn_stages(const GatedNormParams& p, int type, bool backward, int ctas_per_sm) {
+  const uint32_t per_cta = (ctas_per_sm == 1 ? 226 : 113) * 1024u - 600u - gn_extra_bytes(p, backward);
   const uint32_t n = per_cta / gn_stage_bytes(p, type, backward);
   return static_cast<int>(n < GN_RING ? n : GN_RING);
 }
@@ -294,8 +292,10 @@ static int gn_stages(const GatedNormParams& p, int type, bool backward) {
 // Which form: a ring of two stages or more, aligned rows, and more blocks of rows than a CTA would have in one go.
 template <int W>
 static bool gn_takes_ring(GatedNormParams& p, int type, bool backward, uint32_t* smem) {
-  const long long blocks = (p.rows + gn_rows<W>() - 1LL) / gn_rows<W>(), resident = gn_sms() * static_cast<long long>(gn_ctas_per_sm<W>());
-  p.stages = gn_stages(p, type, backward);
+  // Two CTAs per SM where two stages of each fit; 512 threads of the backward kernel take the registers of a whole SM.
+  p.ctas_per_sm = W == 16 && (backward || gn_stages(p, type, backward, 2) < 2) ? 1 : 2;
+  p.stages = gn_stages(p, type, backward, p.ctas_per_sm);
+  const long long blocks = (p.rows + gn_rows<W>() - 1LL) / gn_rows<W>(), resident = gn_sms() * static_cast<long long>(p.ctas_per_sm);
   *smem = p.stages * gn_stage_bytes(p, type, backward) + gn_extra_bytes(p, backward);
   return p.aligned && p.stages >= 2 && blocks >= 2 * resident;
 }

@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const G
 // which the column sums and g w_d take 48.  w is read from shared memory, and so is dw_d for a gate per sequence, which is
 // touched once per sequence.
 template <typename T, int W, int G>
-__global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_norm_bwd_ring_kernel(const GatedNormParams p) {
+__global__ void __launch_bounds__(gn_threads<W>(), W == 16 ? 1 : 2) gated_norm_bwd_ring_kernel(const GatedNormParams p) {
   chain_begin();
   constexpr int R = gn_rows<W>(), V = GN_VECS, THREADS = gn_threads<W>();
   extern __shared__ __align__(128) uint8_t gn_smem[];

@@ -68,12 +68,18 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_fwd_kernel(const G
   }
 }
 
+// Two CTAs per SM, also for rows of more than 4096 values, where 512 threads of 64 registers read the weights from L1 instead of
+// holding them (20011 x 5120 with a gate per element: one CTA 193 us, two 173).
+constexpr int GN_FWD_CTAS = 2;
+
 // One barrier per row: the sum over delta of the next row is formed before the sum over s of the present one, and both cross the
-// warps together.  A CTA has a run of rows, so that a gate per sequence is loaded once per sequence and CTA.
+// warps together.  TB/s of the tensors, gate per channel: 5.2 at 16384 x 4096, 5.3 at 131072 x 512; with a gate per element 5.9 at
+// 20011 x 5120, 6.5 at 12000 x 8192.  More stages and streaming stores gave nothing.
 template <typename T, int W, int G>
-__global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_norm_fwd_ring_kernel(const GatedNormParams p) {
+__global__ void __launch_bounds__(gn_threads<W>(), GN_FWD_CTAS) gated_norm_fwd_ring_kernel(const GatedNormParams p) {
   chain_begin();
   constexpr int R = gn_rows<W>(), V = GN_VECS;
+  constexpr bool HELD = W < 16;                      // the weights are in registers
   extern __shared__ __align__(128) uint8_t gn_smem[];
   __shared__ uint64_t bars[R][GN_RING];
   __shared__ float2 scratch[2][R][W];
@@ -81,19 +87,25 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = warp / W, in_row = warp % W, D = p.D;
   const uint32_t row_bytes = D * sizeof(T), gate_bytes = p.gate_f32 ? D * 4 : row_bytes;
   const uint32_t slot_bytes = 2 * row_bytes + (G == GATE_FULL ? gate_bytes : 0), stage_bytes = R * slot_bytes;
-  const int begin = gn_first_row(blockIdx.x, p.rows, gridDim.x), end = gn_first_row(blockIdx.x + 1, p.rows, gridDim.x);
+  // a run of rows for each CTA where a sequence's gate is loaded, or all CTAs side by side: neighbouring rows are in one DRAM page
+  constexpr bool RUNS = G == GATE_SEQUENCE;
+  const int begin = RUNS ? gn_first_row(blockIdx.x, p.rows, gridDim.x) : static_cast<int>(blockIdx.x) * R;
+  const int end = RUNS ? gn_first_row(blockIdx.x + 1, p.rows, gridDim.x) : p.rows;
+  const int step = RUNS ? R : static_cast<int>(gridDim.x) * R;
   const uint8_t* const mine = gn_smem + slot * slot_bytes;
   const GnRing<3> ring = {{static_cast<const uint8_t*>(p.x), static_cast<const uint8_t*>(p.delta),
                            G == GATE_FULL ? static_cast<const uint8_t*>(p.gate) : nullptr},
                           {row_bytes, row_bytes, gate_bytes}, gn_smem + slot * slot_bytes, stage_bytes, p.stages, bars[slot],
-                          begin + slot, R, end};
+                          begin + slot, step, end};
   const bool leader = in_row == 0 && lane == 0;
   if (leader) ring.start();
   const float inv = 1.f / D;
-  float gwd[V][8], w[V][8];
-  if (G != GATE_SEQUENCE) load_gwd<T, W, G>(p, 0, in_row, lane, gwd);
+  float gwd[HELD ? V : 1][8], w[HELD ? V : 1][8];
+  if constexpr (HELD) {
+    if (G != GATE_SEQUENCE) load_gwd<T, W, G>(p, 0, in_row, lane, gwd);
 #pragma unroll
-  for (int c = 0; c < V; ++c) load_f32x8(p.weight, ((c * W + in_row) * 32 + lane) * 8, D, true, w[c]);
+    for (int c = 0; c < V; ++c) load_f32x8(p.weight, ((c * W + in_row) * 32 + lane) * 8, D, true, w[c]);
+  }
   bool here = true;
   // sum of squares of delta's columns of this lane in a stage that has arrived
   auto squares = [&](int stage) {
@@ -134,10 +146,12 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
   if (begin + slot >= end) return;                   // a slot's warps meet nobody else
   gn_arrived(here, bars[slot][0], 0, p.status, lane);
   float rd = rsqrtf(row_sums(squares(0), 0.f, 1).x * inv + p.eps);
-  for (int row = begin + slot; row < end; row += R, ++turn, half ^= 1) {
-    if (G == GATE_SEQUENCE && row >= sequence_end) {
-      sequence_end = (row / p.seq + 1) * p.seq;
-      load_gwd<T, W, G>(p, row, in_row, lane, gwd);
+  for (int row = begin + slot; row < end; row += step, ++turn, half ^= 1) {
+    if constexpr (HELD && G == GATE_SEQUENCE) {
+      if (row >= sequence_end) {
+        sequence_end = (row / p.seq + 1) * p.seq;
+        load_gwd<T, W, G>(p, row, in_row, lane, gwd);
+      }
     }
     const float token = G == GATE_TOKEN
                             ? (p.gate_f32 ? static_cast<const float*>(p.gate)[row] : to_f32<T>(static_cast<const T*>(p.gate)[row]))
@@ -161,9 +175,19 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[i] *= g[i];
       }
+      float wd[8];
+      if constexpr (!HELD) {
+        load_f32x8(p.delta_weight, col, D, true, wd);
+        if (G == GATE_CHANNEL || G == GATE_SEQUENCE) {
+          float g[8];
+          load_gate<T>(p, row, col, g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) wd[i] *= g[i];
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        s[c][i] = s[c][i] * p.residual_scale + d[i] * factor * gwd[c][i];
+        s[c][i] = s[c][i] * p.residual_scale + d[i] * factor * (HELD ? gwd[HELD ? c : 0][i] : wd[i]);
         sum += s[c][i] * s[c][i];
       }
       Eight<T> out;
@@ -176,7 +200,7 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
       phase ^= 1;
     }
     float next = 0.f;
-    if (row + R < end) {
+    if (row + step < end) {
       gn_arrived(here, bars[slot][stage], phase, p.status, lane);
       next = squares(stage);
     }
@@ -191,8 +215,10 @@ __global__ void __launch_bounds__(gn_threads<W>(), gn_ctas_per_sm<W>()) gated_no
     for (int c = 0; c < V; ++c) {
       const int col = ((c * W + in_row) * 32 + lane) * 8;
       if (col >= D) continue;
+      float wc[8];
+      if constexpr (!HELD) load_f32x8(p.weight, col, D, true, wc);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[c][i] *= r * w[c][i];
+      for (int i = 0; i < 8; ++i) s[c][i] *= r * (HELD ? w[HELD ? c : 0][i] : wc[i]);
       Eight<T> out;
       out.set(s[c]);
       out.store(normed, col, D, true);
@@ -207,7 +233,7 @@ static cudaError_t gn_forward(GatedNormParams& p, int type, cudaStream_t s) {
   constexpr int R = gn_rows<W>(), THREADS = gn_threads<W>();
   uint32_t smem;
   if (gn_takes_ring<W>(p, type, false, &smem)) {
-    const int ctas = gn_sms() * gn_ctas_per_sm<W>();
+    const int ctas = gn_sms() * p.ctas_per_sm;
     switch (p.gate_kind) {
       case GATE_NONE:                // as a gate per channel of ones
       case GATE_CHANNEL: return gn_launch_ring<gated_norm_fwd_ring_kernel<T, W, GATE_CHANNEL>>(ctas, THREADS, smem, s, p);

@@ -95,6 +95,9 @@ def main():
     del hk, wk
     dy = rnd(T, 6144)
     gemm_case("gemm_nn dx 16384x4096x6144", 2 * T * 6144 * D, lambda: native.gemm_nn(dy, wqkv), lambda: dy @ wqkv)
+    (x8, sx8), (w8, sw8), (dy8, sdy8) = native.quantize_fp8(x, 1), native.quantize_fp8(wqkv, 128), native.quantize_fp8(dy, 1)
+    gemm_case("gemm_fp8 qkv 16384x6144x4096, scales of 128", 2 * T * 6144 * D, lambda: native.gemm_fp8(x8, sx8, w8, sw8))
+    gemm_case("gemm_fp8 dx 16384x4096x6144, scales of 128", 2 * T * 6144 * D, lambda: native.gemm_fp8(dy8, sdy8, w8, sw8, nn=True))
     acc = torch.zeros(6144, D, device="cuda")
     gemm_case("gemm_tn dw 6144x4096x16384 (+= fp32)", 2 * T * 6144 * D,
               lambda: native.gemm_tn(dy, x, out=acc, accumulate=True), lambda: acc.addmm_(dy.t().float(), x.float()))
@@ -142,6 +145,20 @@ def main():
     bw_case("add_rmsnorm_fwd 16384x4096", 4 * T * D * 2, lambda: native.add_rmsnorm_fwd(x, x, wn, 1e-5))
     _, rstd = native.rmsnorm_fwd(x, wn, 1e-5)
     bw_case("rmsnorm_bwd 16384x4096", 3 * T * D * 2, lambda: native.rmsnorm_bwd(x, x, wn, rstd))
+    for name, kind, g in (("no gate", 0, None), ("a gate per channel", 1, rnd(D)), ("a gate per value", 4, rnd(T, D))):
+        extra = T * D * 2 * (kind == 4)
+        bw_case(f"gated_norm_fwd 16384x4096, {name}", 4 * T * D * 2 + extra,
+                lambda: native.gated_norm_fwd(x, x, wn, wn, g, kind, 1, 1.0, 1e-5))
+        stats = native.gated_norm_fwd(x, x, wn, wn, g, kind, 1, 1.0, 1e-5)[2]
+        bw_case(f"gated_norm_bwd 16384x4096, {name}", 6 * T * D * 2 + 2 * extra,
+                lambda: native.gated_norm_bwd(x, x, x, x, wn, wn, g, stats, kind, 1, 1.0))
+    bw_case("quantize_fp8 16384x4096 by rows", 3 * T * D, lambda: native.quantize_fp8(x, 1))
+    bw_case("quantize_fp8 16384x4096 by blocks", 3 * T * D, lambda: native.quantize_fp8(x, 128))
+    for experts, k, how in ((64, 6, (False, None, 1, 1, False, False, 1.0)),
+                            (256, 8, (True, torch.zeros(256, device="cuda"), 8, 4, True, True, 2.5))):
+        scores = torch.randn(T, experts, device="cuda")
+        bw_case(f"route_topk 16384 tokens, {k} of {experts} experts", T * (experts * 4 + k * 12),
+                lambda: native.route_topk_fwd(scores, k, *how))
     gate, up = rnd(R, Fd), rnd(R, Fd)
     bw_case("swiglu_bwd 32768x14336", 6 * R * Fd * 2, lambda: native.swiglu_bwd(h, gate, up))
     logits = rnd(T, 32000)

@@ -145,13 +145,14 @@ def main():
     bw_case("add_rmsnorm_fwd 16384x4096", 4 * T * D * 2, lambda: native.add_rmsnorm_fwd(x, x, wn, 1e-5))
     _, rstd = native.rmsnorm_fwd(x, wn, 1e-5)
     bw_case("rmsnorm_bwd 16384x4096", 3 * T * D * 2, lambda: native.rmsnorm_bwd(x, x, wn, rstd))
+    delta, dsum, dnormed = rnd(T, D), rnd(T, D), rnd(T, D)
     for name, kind, g in (("no gate", 0, None), ("a gate per channel", 1, rnd(D)), ("a gate per value", 4, rnd(T, D))):
         extra = T * D * 2 * (kind == 4)
         bw_case(f"gated_norm_fwd 16384x4096, {name}", 4 * T * D * 2 + extra,
-                lambda: native.gated_norm_fwd(x, x, wn, wn, g, kind, 1, 1.0, 1e-5))
-        stats = native.gated_norm_fwd(x, x, wn, wn, g, kind, 1, 1.0, 1e-5)[2]
+                lambda: native.gated_norm_fwd(x, delta, wn, wn, g, kind, 1, 1.0, 1e-5))
+        stats = native.gated_norm_fwd(x, delta, wn, wn, g, kind, 1, 1.0, 1e-5)[2]
         bw_case(f"gated_norm_bwd 16384x4096, {name}", 6 * T * D * 2 + 2 * extra,
-                lambda: native.gated_norm_bwd(x, x, x, x, wn, wn, g, stats, kind, 1, 1.0))
+                lambda: native.gated_norm_bwd(dsum, dnormed, x, delta, wn, wn, g, stats, kind, 1, 1.0))
     bw_case("quantize_fp8 16384x4096 by rows", 3 * T * D, lambda: native.quantize_fp8(x, 1))
     bw_case("quantize_fp8 16384x4096 by blocks", 3 * T * D, lambda: native.quantize_fp8(x, 128))
     for experts, k, how in ((64, 6, (False, None, 1, 1, False, False, 1.0)),

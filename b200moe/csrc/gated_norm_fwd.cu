@@ -68,18 +68,13 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_fwd_kernel(const G
   }
 }
 
-// Two CTAs per SM, also for rows of more than 4096 values, where 512 threads of 64 registers read the weights from L1 instead of
-// holding them (20011 x 5120 with a gate per element: one CTA 193 us, two 173).
-constexpr int GN_FWD_CTAS = 2;
-
 // One barrier per row: the sum over delta of the next row is formed before the sum over s of the present one, and both cross the
-// warps together.  TB/s of the tensors, gate per channel: 5.2 at 16384 x 4096, 5.3 at 131072 x 512; with a gate per element 5.9 at
-// 20011 x 5120, 6.5 at 12000 x 8192.  More stages and streaming stores gave nothing.
+// warps together.  TB/s of the tensors, gate per channel: 5.7 at 16384 x 4096, 5.3 at 131072 x 512; with a gate per element 6.2 at
+// 20011 x 5120 and at 12000 x 8192.  Streaming stores gave nothing.
 template <typename T, int W, int G>
-__global__ void __launch_bounds__(gn_threads<W>(), GN_FWD_CTAS) gated_norm_fwd_ring_kernel(const GatedNormParams p) {
+__global__ void __launch_bounds__(gn_threads<W>(), W == 16 ? 1 : 2) gated_norm_fwd_ring_kernel(const GatedNormParams p) {
   chain_begin();
   constexpr int R = gn_rows<W>(), V = GN_VECS;
-  constexpr bool HELD = W < 16;                      // the weights are in registers
   extern __shared__ __align__(128) uint8_t gn_smem[];
   __shared__ uint64_t bars[R][GN_RING];
   __shared__ float2 scratch[2][R][W];
@@ -100,12 +95,10 @@ __global__ void __launch_bounds__(gn_threads<W>(), GN_FWD_CTAS) gated_norm_fwd_r
   const bool leader = in_row == 0 && lane == 0;
   if (leader) ring.start();
   const float inv = 1.f / D;
-  float gwd[HELD ? V : 1][8], w[HELD ? V : 1][8];
-  if constexpr (HELD) {
-    if (G != GATE_SEQUENCE) load_gwd<T, W, G>(p, 0, in_row, lane, gwd);
+  float gwd[V][8], w[V][8];
+  if (G != GATE_SEQUENCE) load_gwd<T, W, G>(p, 0, in_row, lane, gwd);
 #pragma unroll
-    for (int c = 0; c < V; ++c) load_f32x8(p.weight, ((c * W + in_row) * 32 + lane) * 8, D, true, w[c]);
-  }
+  for (int c = 0; c < V; ++c) load_f32x8(p.weight, ((c * W + in_row) * 32 + lane) * 8, D, true, w[c]);
   bool here = true;
   // sum of squares of delta's columns of this lane in a stage that has arrived
   auto squares = [&](int stage) {
@@ -147,11 +140,9 @@ __global__ void __launch_bounds__(gn_threads<W>(), GN_FWD_CTAS) gated_norm_fwd_r
   gn_arrived(here, bars[slot][0], 0, p.status, lane);
   float rd = rsqrtf(row_sums(squares(0), 0.f, 1).x * inv + p.eps);
   for (int row = begin + slot; row < end; row += step, ++turn, half ^= 1) {
-    if constexpr (HELD && G == GATE_SEQUENCE) {
-      if (row >= sequence_end) {
-        sequence_end = (row / p.seq + 1) * p.seq;
-        load_gwd<T, W, G>(p, row, in_row, lane, gwd);
-      }
+    if (G == GATE_SEQUENCE && row >= sequence_end) {
+      sequence_end = (row / p.seq + 1) * p.seq;
+      load_gwd<T, W, G>(p, row, in_row, lane, gwd);
     }
     const float token = G == GATE_TOKEN
                             ? (p.gate_f32 ? static_cast<const float*>(p.gate)[row] : to_f32<T>(static_cast<const T*>(p.gate)[row]))
@@ -175,19 +166,9 @@ __global__ void __launch_bounds__(gn_threads<W>(), GN_FWD_CTAS) gated_norm_fwd_r
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[i] *= g[i];
       }
-      float wd[8];
-      if constexpr (!HELD) {
-        load_f32x8(p.delta_weight, col, D, true, wd);
-        if (G == GATE_CHANNEL || G == GATE_SEQUENCE) {
-          float g[8];
-          load_gate<T>(p, row, col, g);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) wd[i] *= g[i];
-        }
-      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        s[c][i] = s[c][i] * p.residual_scale + d[i] * factor * (HELD ? gwd[HELD ? c : 0][i] : wd[i]);
+        s[c][i] = s[c][i] * p.residual_scale + d[i] * factor * gwd[c][i];
         sum += s[c][i] * s[c][i];
       }
       Eight<T> out;
@@ -215,10 +196,8 @@ __global__ void __launch_bounds__(gn_threads<W>(), GN_FWD_CTAS) gated_norm_fwd_r
     for (int c = 0; c < V; ++c) {
       const int col = ((c * W + in_row) * 32 + lane) * 8;
       if (col >= D) continue;
-      float wc[8];
-      if constexpr (!HELD) load_f32x8(p.weight, col, D, true, wc);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[c][i] *= r * (HELD ? w[HELD ? c : 0][i] : wc[i]);
+      for (int i = 0; i < 8; ++i) s[c][i] *= r * w[c][i];
       Eight<T> out;
       out.set(s[c]);
       out.store(normed, col, D, true);
@@ -242,7 +221,7 @@ static cudaError_t gn_forward(GatedNormParams& p, int type, cudaStream_t s) {
       default: return gn_launch_ring<gated_norm_fwd_ring_kernel<T, W, GATE_FULL>>(ctas, THREADS, smem, s, p);
     }
   }
-  const long long blocks = (p.rows + R - 1LL) / R, most = gn_sms() * (W == 16 ? 4LL : 8LL);
+  const long long blocks = (p.rows + R - 1LL) / R, most = gn_sms() * (W > 8 ? 4LL : 8LL);
   return launch_next(gated_norm_fwd_kernel<T, W>, static_cast<unsigned>(blocks < most ? blocks : most), THREADS, 0, s, p);
 }
 
@@ -261,7 +240,7 @@ int b2_gated_norm_fwd(const void* x, const void* delta, const float* delta_weigh
   p.x = x; p.delta = delta; p.delta_weight = delta_weight; p.weight = weight; p.gate = gate; p.summed = summed;
   p.normed = normed; p.delta_rstd = delta_rstd; p.rstd = rstd; p.rows = rows; p.D = D; p.seq = seq;
   p.gate_kind = gate_kind; p.gate_f32 = gate_f32; p.residual_scale = residual_scale; p.status = status; p.eps = eps;
-  return gated_norm(p, type, [&](auto tag, auto width) { return gn_forward<decltype(tag), decltype(width)::value>(p, type, s); });
+  return gated_norm<false>(p, type, [&](auto tag, auto width) { return gn_forward<decltype(tag), decltype(width)::value>(p, type, s); });
 }
 
 }  // extern "C"

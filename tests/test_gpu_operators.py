@@ -218,6 +218,15 @@ def test_gated_add_rmsnorm_of_many_rows(B, S, D, dtype, kind):
         _check_norm(*_norm_case(B, S, D, kind, dtype, torch.float32), use=(D == 2048, D != 2048))
 
 
+@pytest.mark.parametrize("kind", ["none", "channel", "sequence", "token", "full"])
+@pytest.mark.parametrize("B,S,D,dtype", [(2, 307, 4104, torch.bfloat16), (11, 83, 6144, torch.bfloat16), (1, 900, 4608, torch.float16),
+                                         (1, 617, 4224, torch.float32), (1, 611, 6136, torch.float32), (2, 350, 6152, torch.bfloat16)])
+def test_gated_add_rmsnorm_of_ten_and_twelve_warps(B, S, D, dtype, kind):
+    _check_norm(*_norm_case(B, S, D, kind, dtype))
+    if dtype != torch.float32:
+        _check_norm(*_norm_case(B, S, D, kind, dtype, torch.float32))
+
+
 def test_gated_add_rmsnorm_uses_and_layouts():
     for use in ((True, False), (False, True)):
         _check_norm(*_norm_case(2, 30, 264, "channel", torch.bfloat16), use=use)

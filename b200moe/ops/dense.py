@@ -310,6 +310,8 @@ def gated_add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, delta_weight: torch.
         return Fn.gated_add_rmsnorm_ref(x, delta, delta_weight, weight, gate, residual_scale, eps)
     if not 1 <= width <= 8192:
         raise ValueError(f"rows of 1 to 8192 values, got {width}")
+    if x.numel() // width >= 2 ** 31 - 1:
+        raise ValueError(f"at most 2^31 - 2 rows, got {x.numel() // width}")
     seq = x.numel() // max(x.shape[0] * width, 1) if kind == 2 else 1
     args = (x, delta, delta_weight, weight, gate, kind, max(seq, 1), float(residual_scale), float(eps))
     if backward_follows(x, delta, delta_weight, weight, gate):

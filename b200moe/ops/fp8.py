@@ -12,6 +12,11 @@ from torch.autograd.function import once_differentiable
 from . import backward_follows, cpp_nodes, functional as Fn, native, use_native
 
 
+def _check_size(name: str, x) -> None:
+    if max(x.shape) > 2 ** 31 - 128:
+        raise ValueError(f"{name} {list(x.shape)} has more than 2^31 - 128 rows or columns")
+
+
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
     """``(values e4m3 [M, K], scales fp32)`` of ``x [M, K]`` (fp32, bf16 or fp16).  ``block_rows`` 1: a scale for each row and
     128 columns, ``[M, ceil(K / 128)]``; 128: one for each 128 x 128 values, ``[ceil(M / 128), ceil(K / 128)]``.  A scale is
@@ -19,6 +24,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
     multiples of 16 bytes, as ``matmul_fp8`` reads them.  NaN stays NaN; a block with an infinity has an infinite scale."""
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be [rows, columns] with a column at least, got {list(x.shape)}")
+    _check_size("x", x)
     if block_rows not in (1, 128):
         raise ValueError(f"block_rows must be 1 or 128, got {block_rows}")
     if not x.dtype.is_floating_point:
@@ -31,6 +37,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
 def _check_operand(name: str, values, scales, block_rows: int) -> None:
     if values.dim() != 2 or min(values.shape[1], 1) < 1 or values.dtype != torch.float8_e4m3fn:
         raise TypeError(f"{name} must be float8_e4m3fn [rows, columns], got {values.dtype} {list(values.shape)}")
+    _check_size(name, values)
     want = ((values.shape[0] + block_rows - 1) // block_rows, (values.shape[1] + 127) // 128)
     if scales.dtype != torch.float32 or tuple(scales.shape) != want or scales.device != values.device:
         raise ValueError(f"the scales of {name} {list(values.shape)} must be fp32 {list(want)} on {values.device}, got "
@@ -125,6 +132,9 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_fp8=None) -> torch.
             return out
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
         raise ValueError(f"x {list(x.shape)} and weight {list(weight.shape)} must share their last dimension, and the weight have a row")
+    _check_size("weight", weight)
+    if x.numel() // x.shape[-1] > 2 ** 31 - 128:
+        raise ValueError(f"x {list(x.shape)} has more than 2^31 - 128 rows")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
     if getattr(weight, "pending_gather", None) is not None:

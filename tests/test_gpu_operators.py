@@ -444,6 +444,17 @@ def test_linear_fp8_of_widths_that_have_no_gradient_products():
     _check_product(dx, torch.ones(9, 77, device="cuda", dtype=torch.float64), exact[1].t())
 
 
+def test_rows_beyond_32_bits_are_refused():
+    one, w = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16), torch.ones(1, device="cuda")
+    many = one.expand(2 ** 31, 1)
+    with pytest.raises(ValueError, match="rows"):
+        ops.gated_add_rmsnorm(many, many, w, w)
+    with pytest.raises(ValueError, match="rows"):
+        ops.quantize_fp8(many)
+    with pytest.raises(ValueError, match="rows"):
+        ops.linear_fp8(many, one)
+
+
 def test_fp8_refuses_on_the_gpu():
     a, sa = _operand(5, 200, 1)
     b, sb = _operand(7, 200, 128)

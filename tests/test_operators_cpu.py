@@ -142,6 +142,17 @@ def test_linear_fp8_statement_and_gradients():
     assert torch.allclose(w.main_grad, 1 + dw, rtol=1e-5, atol=1e-5)
 
 
+def test_fp8_refuses_sizes_beyond_32_bits():
+    long = torch.zeros(1, 1, dtype=torch.bfloat16)
+    for shape in ((2 ** 31, 1), (1, 2 ** 32 + 128)):
+        with pytest.raises(ValueError, match="rows or columns"):
+            ops.quantize_fp8(long.expand(shape))
+        with pytest.raises(ValueError, match="rows or columns"):
+            ops.matmul_fp8(long.to(torch.float8_e4m3fn).expand(shape), torch.ones(1, 1), *ops.quantize_fp8(long, 128))
+    with pytest.raises(ValueError, match="rows"):
+        ops.linear_fp8(long.expand(2 ** 31, 1), long)
+
+
 def test_fp8_refuses():
     q, s = ops.quantize_fp8(torch.randn(5, 200), 1)
     b, t = ops.quantize_fp8(torch.randn(7, 200), 128)

@@ -229,7 +229,8 @@ def quantize_fp8_ref(x: torch.Tensor, block_rows: int = 1):
     rows, cols = x.shape
     blocks = _fp8_blocks(x, block_rows)
     most = torch.where(torch.isnan(blocks), 0.0, blocks.abs()).amax((1, 3))
-    scales = (most / E4M3_MAX).clamp(min=SMALLEST_FP8_SCALE)
+    # by a tensor: a division by a number is a product with its rounded reciprocal on a GPU, which half of the scales differ by
+    scales = (most / torch.full_like(most, E4M3_MAX)).clamp(min=SMALLEST_FP8_SCALE)
     values = (blocks / scales[:, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
     return values.view(blocks.shape[0] * block_rows, blocks.shape[2] * 128)[:rows, :cols].contiguous(), scales
 

@@ -386,25 +386,35 @@ __device__ __forceinline__ int choose(const RouteParams& p, long long row, const
     const uint32_t key_after = __shfl_down_sync(ALL, my_key, 1);
     const int index_after = __shfl_down_sync(ALL, index, 1);
     const float ka = unordered(my_key), kb = unordered(lane == LANES - 1 ? extra : key_after);
-    bool near = lane < steps - 1 && kb != -INFINITY && ka - kb <= key_error(most, ka, p.sigmoid) + key_error(most, kb, p.sigmoid);
+    const bool near = lane < steps - 1 && kb != -INFINITY && ka - kb <= key_error(most, ka, p.sigmoid) + key_error(most, kb, p.sigmoid);
+    bool doubtful = near;
     float xa = 0.f, xb = 0.f, ba = 0.f, bb = 0.f;
     if (near && lane != LANES - 1) {                // equal experts are in the order of their indices
       xa = load_logit(p.logits, p.type, row * p.E + index);
       xb = load_logit(p.logits, p.type, row * p.E + index_after);
       ba = p.bias[index];
       bb = p.bias[index_after];
-      near = !(xa == xb && ba == bb);
+      doubtful = !(xa == xb && ba == bb);
     }
-    const unsigned doubtful = row_ballot<LANES>(near);
-    // Sigmoids of a pair whose neighbours are not in doubt are put in order in 64 bits on the spot.  Softmaxes, which need all
-    // logits again, and runs of close keys are left to the row's second pass.
-    const bool alone = near && p.sigmoid && lane != LANES - 1 && !((doubtful << 1 | doubtful >> 1) >> lane & 1);
+    // Near pairs that follow one another are a run, equal ones among them: what belongs in front of one of two equal experts belongs
+    // in front of both.  Sigmoids of a pair that is a run by itself are put in order in 64 bits on the spot.  Softmaxes, which need
+    // all logits again, and longer runs are left to the row's second pass where they reach the first k.
+    const unsigned nears = row_ballot<LANES>(near);
+    const bool alone = doubtful && p.sigmoid && lane != LANES - 1 && !((nears << 1 | nears >> 1) >> lane & 1);
     bool swap = false;
     if (alone) {
       const double a = 1.0 / (1.0 + exp(-static_cast<double>(xa))) + ba, b = 1.0 / (1.0 + exp(-static_cast<double>(xb))) + bb;
       swap = b > a || (a == b && index_after < index);
     }
-    close |= near && lane < p.k && !alone;
+    // the run that leaves the first k between their last pair and the one behind it
+    const bool leaves = p.k < LANES && (nears >> (p.k - 1) & nears >> p.k & 1);
+    close |= doubtful && !alone && (lane < p.k || (lane == p.k && leaves));
+    if (__any_sync(ALL, leaves && steps < candidates)) {      // it may go on behind the last key that was looked at
+      const float next = unordered(row_max<LANES>(h[0]));
+      const float last = unordered(__shfl_sync(ALL, my_key, min(steps - 1, LANES - 1), LANES));
+      close |= leaves && steps < candidates && next != -INFINITY &&
+               last - next <= key_error(most, last, p.sigmoid) + key_error(most, next, p.sigmoid);
+    }
     const unsigned swaps = row_ballot<LANES>(swap);
     const int index_before = __shfl_up_sync(ALL, index, 1);
     if (swaps >> lane & 1) index = index_after;

@@ -1,7 +1,10 @@
 """Routing, gated residual norm and 8-bit products on the GPU where equal, close, far and empty operands meet."""
+import itertools
+
 import pytest
 import torch
 
+import _operators as want
 from b200moe import ops
 
 pytestmark = pytest.mark.gpu
@@ -14,6 +17,52 @@ def _native():
     torch.manual_seed(12)
     yield
     native.check_status()
+
+
+# ------------------------------------------------------------------------------ choice among equal and close experts
+def _close_rows(E, front, others):
+    """A row for each order of the logits ``front``, next to each other and spread over the experts; the others are far behind."""
+    orders = sorted(set(itertools.permutations(front))) if len(front) <= 4 else [tuple(front), tuple(reversed(front))]
+    rows = []
+    for order in orders:
+        for step in sorted({1, max(1, (E - 1) // max(len(front) - 1, 1))}):
+            row = [others - 0.25 * i / E for i in range(E)]
+            for i, v in enumerate(order):
+                row[i * step] = v
+            rows.append(row)
+    return torch.tensor(rows)
+
+
+@pytest.mark.parametrize("score,front,others,bias", [
+    ("sigmoid", [17.0, 17.0, 17.125], -5.0, 0.0), ("sigmoid", [18.0, 18.0, 18.125, 18.125], -5.0, 0.0),
+    ("sigmoid", [17.0, 17.125, 17.25, 17.375], -5.0, 0.5), ("sigmoid", [17.0, 17.0, 17.0, 17.125], -5.0, -0.25),
+    ("sigmoid", [17.0] * 7 + [17.125], -5.0, 0.0), ("sigmoid", [17.125] + [17.0] * 6 + [17.125], -5.0, 0.0),
+    ("softmax", [0.0, 0.0, 0.0078125], -20.0, 1.0), ("softmax", [0.0, 0.0078125, 0.0078125, 0.0], -20.0, 1.0),
+    ("softmax", [0.0] * 7 + [0.0078125], -20.0, 1.0)])
+def test_close_experts_among_equal_ones(score, front, others, bias):
+    for E, k in ((9, 1), (12, 2), (9, 7), (64, 3), (64, 8), (256, 1), (256, 4), (300, 31), (1000, 32)):
+        logits = _close_rows(E, front, others)
+        biases = torch.full((E,), bias)
+        if score == "softmax":                          # one takes nearly all of the sum, so that the others' scores are close
+            logits[:, E - 1] = 17.0
+            biases[E - 1] = 0.0
+        for dtype in (torch.float32, torch.bfloat16):
+            x = logits.to(dtype)
+            _, idx = ops.route_topk(x.cuda(), k, score=score, bias=biases.cuda())
+            assert torch.equal(idx.cpu(), want.route(x, k, score=score, bias=biases)[1]), (E, k, dtype)
+
+
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (4, 2)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_repeated_logits_and_biases(score, groups, top_groups):
+    """Few different logits, saturated or not, and few different biases: equal and close keys everywhere."""
+    T, E = 400, 64
+    x = torch.randint(0, 4, (T, E)) * 0.125 + torch.tensor([0.0, 4.0, 17.0, 20.0])[torch.randint(0, 4, (T, 1))]
+    bias = torch.randint(0, 2, (E,)) * 2.0 ** -22
+    for k in (1, 6, 9):
+        how = dict(score=score, bias=bias, groups=groups, top_groups=top_groups)
+        _, idx = ops.route_topk(x.bfloat16().cuda(), k, **{**how, "bias": bias.cuda()})
+        assert torch.equal(idx.cpu(), want.route(x.bfloat16(), k, **how)[1])
 
 
 # ------------------------------------------------------------------------------ 8-bit values

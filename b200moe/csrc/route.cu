@@ -306,14 +306,13 @@ __device__ __forceinline__ int choose(const RouteParams& p, long long row, const
     }
     allowed = row_ballot<LANES>(group && in_front < p.top_groups);
     if (scored) {
-      // the last group that stays against the first that goes
-      const unsigned last = row_ballot<LANES>(group && in_front == p.top_groups - 1);
-      const unsigned next = row_ballot<LANES>(group && in_front == p.top_groups);
-      const float a = __shfl_sync(ALL, value, __ffs(last) - 1, LANES), b = __shfl_sync(ALL, value, __ffs(next) - 1, LANES);
-      // the sum of two keys rounds once more; a key is below its group's sum plus one in size
-      const float terms = p.two_best ? 2.f : 1.f;
-      const float error = terms * (key_error(most, fabsf(a) + 1.f, p.sigmoid) + key_error(most, fabsf(b) + 1.f, p.sigmoid));
-      close = b != -INFINITY && a - b <= error;
+      // Each group that stays against each that goes.  A key is off by what its own size says, which the sum of two of opposite signs
+      // hides.  The sum rounds once more, and so do its bounds: by a step of the sum each, at most two of the larger key.
+      const float reach = value == -INFINITY ? 0.f : fmaxf(fabsf(best), p.two_best && second != -INFINITY ? fabsf(second) : 0.f);
+      const float error = (p.two_best ? 2.f : 1.f) * key_error(most, 3.f * reach, p.sigmoid);
+      const bool stays = group && in_front < p.top_groups, goes = group && !stays && value != -INFINITY;
+      const float low = row_max_f<LANES>(stays ? error - value : -INFINITY), high = row_max_f<LANES>(goes ? value + error : -INFINITY);
+      close = high != -INFINITY && !(-low > high);
     }
   }
   // Without a bias experts are compared by their logits, whatever the groups were compared by.

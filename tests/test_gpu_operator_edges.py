@@ -65,6 +65,27 @@ def test_repeated_logits_and_biases(score, groups, top_groups):
         assert torch.equal(idx.cpu(), want.route(x.bfloat16(), k, **how)[1])
 
 
+@pytest.mark.parametrize("biases,top_groups", [([40.0, -40.0, 40.0, -40.0], 1), ([1000.0, -1000.0, 0.5, 0.5], 1),
+                                               ([3000.0, -3000.0, 0.25, 0.25, 0.0, 0.0], 2)])
+def test_groups_by_two_keys_of_opposite_signs(biases, top_groups):
+    """The keys round to steps of their own size, which their sum hides."""
+    E = len(biases)
+    T = 3000
+    bias = torch.tensor(biases)
+    x = torch.randn(T, E)
+    value = (torch.sigmoid(x.double()) + bias.double()).view(T, E // 2, 2).sum(2)
+    # the last expert's score makes the sums of its group and of the one before nearly equal
+    room = torch.rand(T, dtype=torch.float64) * 2e-5 - 1e-5
+    score = (torch.sigmoid(x[:, -1].double()) + value[:, -2] - value[:, -1] + room).clamp(0.001, 0.999)
+    x[:, -1] = torch.log(score / (1 - score)).float()
+    if E == 6:                                          # and the first group's, whose keys are the large ones
+        score = (torch.sigmoid(x[:, 0].double()) + value[:, -2] - value[:, 0] + room.flip(0)).clamp(0.001, 0.999)
+        x[:, 0] = torch.log(score / (1 - score)).float()
+    how = dict(score="sigmoid", groups=E // 2, top_groups=top_groups, group_score=2)
+    _, idx = ops.route_topk(x.cuda(), 2 * top_groups, bias=bias.cuda(), **how)
+    assert torch.equal(idx.cpu(), want.route(x, 2 * top_groups, bias=bias, **how)[1])
+
+
 # ------------------------------------------------------------------------------ 8-bit values
 def test_quantize_fp8_statement_on_the_gpu_is_that_on_the_cpu():
     from b200moe.ops import functional as Fn

@@ -555,12 +555,13 @@ __global__ void __launch_bounds__(route_warps(V) * 32, 4) route_fwd_kernel(const
   const float xe = on ? load_logit(p.logits, p.type, row * p.E + e) : -INFINITY;
   float w;
   if (p.renormalize) {
-    // softmax: the other experts cancel.  Sigmoids below -60 are exp(x) to the last bit, and their sum could vanish.
-    const float top = row_max_f<LANES>(xe);
-    if (!p.sigmoid || top < -60.f) w = xe == -INFINITY ? 0.f : expf(xe - top);
-    else w = xe == -INFINITY ? 0.f : __fdividef(1.f, 1.f + expf(-xe));       // 2 units in the last place
+    // Softmax: the other experts cancel.  Sigmoids of negative logits are exp(x) / (1 + exp(x)), all over exp(top) where none is positive: a
+    // score that fp32 does not hold may have a weight that it does.
+    const float top = row_max_f<LANES>(xe), off = p.sigmoid ? fminf(top, 0.f) : top;
+    w = xe == -INFINITY ? 0.f : expf((p.sigmoid ? fminf(xe, 0.f) : xe) - off);
+    if (p.sigmoid) w /= 1.f + expf(-fabsf(xe));
     const float total = row_add<LANES>(w);
-    w = total == 0.f ? 0.f : __fdividef(w, total);
+    w = total == 0.f ? 0.f : w / total;
   } else {
     RowStats st = {0.f, 1.f};
     if (!p.sigmoid) st = softmax_stats<LANES, false, V>(x);

@@ -86,6 +86,27 @@ def test_groups_by_two_keys_of_opposite_signs(biases, top_groups):
     assert torch.equal(idx.cpu(), want.route(x, 2 * top_groups, bias=bias, **how)[1])
 
 
+def test_renormalised_sigmoids_far_apart():
+    """Scores of one row over all of fp32's range: none vanishes that its type holds."""
+    rows = [[-50.0, -90.0, -55.0], [0.0, -85.0, -100.0], [-59.0, -61.0, -130.0], [-100.0, -120.0, -180.0], [30.0, -87.0, 2.0],
+            [-10.0, -95.0, -30.0], [3e38, -3.0, -88.0], [-1.0, 1.0, -1.5], [-200.0, -200.0, -201.0]]
+    x = torch.tensor(rows)
+    leaf = x.cuda().requires_grad_()
+    weights, idx = ops.route_topk(leaf, 3, score="sigmoid")
+    w, i = want.route(x, 3, score="sigmoid")
+    assert torch.equal(idx.cpu(), i)
+    # the difference of two logits is rounded (at most 100 steps of 2^-24 of its exponential), some ten more operations; below 2^-126 steps of 2^-149
+    room = 128 * 2.0 ** -24 * w + 4 * 2.0 ** -149
+    assert bool(((weights.detach().double().cpu() - w).abs() <= room).all())
+    g = torch.randn(len(rows), 3)
+    (got,) = torch.autograd.grad(weights, leaf, g.cuda())
+    exact = want.route_gradient(x, i, g, "sigmoid", True, 1.0)
+    # w_i (1 - s_i) (g_i - sum g w): relative to the weight, whose own room is above
+    v = torch.zeros_like(exact).scatter_(1, i, w)
+    size = v * (g.abs().double().sum(1, keepdim=True) + 1)
+    assert bool(((got.double().cpu() - exact).abs() <= 256 * 2.0 ** -24 * size + 2.0 ** -146).all())
+
+
 # ------------------------------------------------------------------------------ 8-bit values
 def test_quantize_fp8_statement_on_the_gpu_is_that_on_the_cpu():
     from b200moe.ops import functional as Fn

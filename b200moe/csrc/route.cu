@@ -573,10 +573,10 @@ __global__ void __launch_bounds__(route_warps(V) * 32, 4) route_fwd_kernel(const
   }
 }
 
-// Gradient of the logits.  With the weights w = scale * v and their gradient g:
-//   sigmoid, renormalised   v_i (1 - s_i) (scale g_i - sum_j scale g_j v_j)          sigmoid      scale g_i v_i (1 - s_i)
-//   softmax, renormalised   v_i (scale g_i - sum_j scale g_j v_j)                    softmax      the same over all experts
-// for the chosen experts i; the others have none, but for a softmax over all experts: -p_e sum_j scale g_j v_j.
+// Gradient of the logits.  With the weights w, which hold the scale, and their gradient g:
+//   sigmoid, renormalised   w_i (1 - s_i) (g_i - sum_j g_j w_j / scale)              sigmoid      w_i (1 - s_i) g_i
+//   softmax, renormalised   w_i (g_i - sum_j g_j w_j / scale)                        softmax      w_i g_i - p_i sum_j g_j w_j
+// for the chosen experts i; the others have none, but for a softmax over all experts: -p_e sum_j g_j w_j.
 template <int LANES, int V>
 __global__ void __launch_bounds__(route_warps(V) * 32) route_bwd_kernel(const RouteParams p, const float* __restrict__ dweights,
                                                                        void* __restrict__ dlogits) {
@@ -592,12 +592,12 @@ __global__ void __launch_bounds__(route_warps(V) * 32) route_bwd_kernel(const Ro
   const bool on = lane < p.k;
   const long long at = row * p.k + lane;
   const int e = on ? min(max(static_cast<int>(p.idx[at]), 0), p.E - 1) : 0;
-  const float v = on ? p.weights[at] / p.scale : 0.f;
-  float g = on ? dweights[at] * p.scale : 0.f;
+  const float w = on ? p.weights[at] : 0.f;
+  float g = on ? dweights[at] : 0.f;
   const bool all = !p.sigmoid && !p.renormalize;
-  const float inner = row_add<LANES>(g * v);
-  if (p.renormalize) g -= inner;
-  g *= v;
+  const float inner = row_add<LANES>(g * w);
+  if (p.renormalize) g -= inner / p.scale;
+  g *= w;
   if (p.sigmoid && on) g *= 1.f / (1.f + expf(load_logit(p.logits, p.type, row * p.E + e)));
   float prob[V];
 #pragma unroll
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(route_warps(V) * 32) route_bwd_kernel(const Ro
 #pragma unroll
   for (int j = 0; j < V; ++j) out[j * LANES + lane] = 0.f;
   __syncwarp();
-  if (on && v != 0.f) out[e % V * LANES + e / V] = g;          // the place of expert e: its lane is e / V
+  if (on && w != 0.f) out[e % V * LANES + e / V] = g;          // the place of expert e: its lane is e / V
   __syncwarp();
   if (mine >= p.T) return;
   const int first = lane * V;

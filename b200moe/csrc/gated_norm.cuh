@@ -31,6 +31,7 @@ namespace b2 {
 
 constexpr int GN_VECS = 2;                   // runs of 8 columns per lane
 constexpr int GN_MAX_D = 8192;
+constexpr int GN_MAX_ROWS = 0x7fffffff - 0xffff;      // 2^31 - 2^16: a CTA's count of rows goes up to the ring's length beyond the last one
 
 enum GateKind : int { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_SEQUENCE = 2, GATE_TOKEN = 3, GATE_FULL = 4 };
 
@@ -326,7 +327,7 @@ static cudaError_t gn_launch_ring(int ctas, int threads, uint32_t smem, cudaStre
 // Checks and fills ``p`` up, then calls ``launch(type tag, width tag)``.
 template <bool BACKWARD, typename Launch>
 static int gated_norm(GatedNormParams& p, int type, Launch&& launch) {
-  if (p.rows < 0 || p.D < 1 || p.D > GN_MAX_D || type < 0 || type > 2 || p.gate_kind < 0 || p.gate_kind > 4 ||
+  if (p.rows < 0 || p.rows > GN_MAX_ROWS || p.D < 1 || p.D > GN_MAX_D || type < 0 || type > 2 || p.gate_kind < 0 || p.gate_kind > 4 ||
       (p.gate_kind == GATE_SEQUENCE && (p.seq < 1 || p.rows % p.seq)) || (p.gate_kind != GATE_NONE && !p.gate))
     return -10;
   if (p.rows == 0) return 0;

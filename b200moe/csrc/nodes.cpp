@@ -626,7 +626,7 @@ std::optional<variable_list> gated_norm(const Tensor& x, const Tensor& delta, co
         delta.scalar_type() == x.scalar_type() && delta.is_contiguous() && delta.device() == x.device() && std::isfinite(scale) && eps > 0))
     return std::nullopt;
   const int64_t D = x.size(-1);
-  if (!(D <= 8192 && x.numel() / D < INT_MAX)) return std::nullopt;
+  if (!(D <= 8192 && x.numel() / D <= INT_MAX - 0xffff)) return std::nullopt;
   for (const Tensor& t : {wd, w})
     if (!(t.dim() == 1 && t.size(0) == D && t.scalar_type() == at::kFloat && t.is_contiguous() && t.device() == x.device()))
       return std::nullopt;

@@ -284,8 +284,8 @@ def gated_add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, delta_weight: torch.
     """The seam between two blocks with norms on both sides: ``summed = residual_scale · x + gate · rmsnorm(delta,
     delta_weight)`` and ``rmsnorm(summed, weight)``, the latter of the sum before it is rounded; returns both.
 
-    ``x`` and ``delta`` ``[..., D]`` have one type (bf16, fp16 or fp32; D up to 8192).  ``gate``, of that type or fp32, has
-    the shape ``[D]``, ``[B, 1, D]`` for ``x [B, S, D]``, ``[..., 1]`` or that of ``x``."""
+    ``x`` and ``delta`` ``[..., D]`` have one type (on a GPU bf16, fp16 or fp32, D up to 8192, up to 2^31 - 2^16 rows).
+    ``gate``, of that type or fp32, has the shape ``[D]``, ``[B, 1, D]`` for ``x [B, S, D]``, ``[..., 1]`` or that of ``x``."""
     if use_native(x, "gated_norm"):
         nodes = cpp_nodes(x, delta, delta_weight, weight, *(() if gate is None else (gate,)))
         out = nodes.gated_norm(x, delta, delta_weight, weight, gate, residual_scale, eps, native.status_word(x.device)) \
@@ -310,8 +310,8 @@ def gated_add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, delta_weight: torch.
         return Fn.gated_add_rmsnorm_ref(x, delta, delta_weight, weight, gate, residual_scale, eps)
     if not 1 <= width <= 8192:
         raise ValueError(f"rows of 1 to 8192 values, got {width}")
-    if x.numel() // width >= 2 ** 31 - 1:
-        raise ValueError(f"at most 2^31 - 2 rows, got {x.numel() // width}")
+    if x.numel() // width > 2 ** 31 - 2 ** 16:
+        raise ValueError(f"at most 2^31 - 2^16 rows, got {x.numel() // width}")
     seq = x.numel() // max(x.shape[0] * width, 1) if kind == 2 else 1
     args = (x, delta, delta_weight, weight, gate, kind, max(seq, 1), float(residual_scale), float(eps))
     if backward_follows(x, delta, delta_weight, weight, gate):

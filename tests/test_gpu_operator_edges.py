@@ -107,6 +107,18 @@ def test_renormalised_sigmoids_far_apart():
     assert bool(((got.double().cpu() - exact).abs() <= 256 * 2.0 ** -24 * size + 2.0 ** -146).all())
 
 
+# ------------------------------------------------------------------------------ sizes
+def test_gated_norm_refuses_rows_whose_counters_would_overflow():
+    one, w = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16), torch.ones(1, device="cuda")
+    for rows in (2 ** 31 - 2 ** 16 + 1, 2 ** 31 - 2):
+        many = one.expand(rows, 1)
+        with pytest.raises(ValueError, match="rows"):
+            ops.gated_add_rmsnorm(many, many, w, w)
+        many = torch.empty(rows, 1, device="cuda", dtype=torch.bfloat16)      # contiguous: through the C++ node
+        with pytest.raises(ValueError, match="rows"):
+            ops.gated_add_rmsnorm(many, many, w, w)
+
+
 # ------------------------------------------------------------------------------ 8-bit values
 def test_quantize_fp8_statement_on_the_gpu_is_that_on_the_cpu():
     from b200moe.ops import functional as Fn

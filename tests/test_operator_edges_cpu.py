@@ -1,0 +1,37 @@
+"""Routing, gated residual norm and 8-bit products: sizes and operands at the edge of what they take."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+I, L, F, P = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
+REFUSED = -10
+
+
+@pytest.fixture
+def library():
+    """The kernels' library without a GPU, where a call that it does not refuse fails at its launch and starts nothing."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "b200moe", "_C", "libb200moe.so")
+    if torch.cuda.is_available() or not os.path.exists(path):
+        pytest.skip("for a machine without a GPU and with the library built")
+    try:
+        return ctypes.CDLL(path)
+    except OSError as error:
+        pytest.skip(str(error))
+
+
+def test_gated_norm_refuses_rows_whose_counters_would_overflow(library):
+    null = P(None)
+
+    def forward(rows, D):
+        return library.b2_gated_norm_fwd(*[null] * 9, I(rows), I(D), I(1), I(1), I(0), I(0), F(1), F(1e-5), null, null)
+
+    def backward(rows, D):
+        return library.b2_gated_norm_bwd(*[null] * 15, I(rows), I(D), I(1), I(1), I(0), I(0), F(1), null, null)
+
+    for call in (forward, backward):
+        for D in (1, 8):
+            for rows in (2 ** 31 - 2 ** 16 + 1, 2 ** 31 - 2, 2 ** 31 - 1):
+                assert call(rows, D) == REFUSED
+            assert call(2 ** 31 - 2 ** 16, D) != REFUSED

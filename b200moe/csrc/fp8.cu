@@ -37,6 +37,7 @@ constexpr int F8_EVEN = 168, F8_FEW = 72, F8_MANY = 216;
 constexpr int F8_GROUP_M = 8;
 constexpr int F8_AHEAD = 4;
 constexpr int F8_STAGING = F8_EPI_WARPS * 2048;
+constexpr int F8_MAX = 0x7fffffff - 255;       // rows and columns: their counts are rounded up to whole tiles
 
 // ------------------------------------------------------------------ quantisation
 enum QuantType : int { QUANT_F32 = 0, QUANT_BF16 = 1, QUANT_F16 = 2 };
@@ -622,7 +623,7 @@ extern "C" {
 // block_rows 1: [ceil(K / 128), scale_pitch], the scale of row m in column m; 128: [ceil(M / 128), ceil(K / 128)].
 int b2_quantize_fp8(const void* x, int type, void* q, float* scales, long long M, int K, long long ldx, long long pitch,
                     long long scale_pitch, int block_rows, cudaStream_t s) {
-  if (M < 0 || M > 0x7fffffff || K < 1 || pitch < K || pitch % 16 || pitch - K >= 128 || type < 0 || type > 2 ||
+  if (M < 0 || M > F8_MAX || K < 1 || K > F8_MAX || pitch < K || pitch % 16 || pitch - K >= 128 || type < 0 || type > 2 ||
       (block_rows != 1 && block_rows != 128))
     return -10;
   if (M == 0) return 0;
@@ -642,7 +643,7 @@ int b2_quantize_fp8(const void* x, int type, void* q, float* scales, long long M
 int b2_gemm_fp8(const void* a, const float* a_scales, const void* w, const float* b_scales, void* d, int M, int N, int K,
                 long long lda, long long ldw, long long a_row, long long a_block, long long b_row, long long b_block, int nn,
                 int* status, cudaStream_t s) {
-  if (M < 0 || N < 1 || K < 1 || lda % 16 || ldw % 16) return -10;
+  if (M < 0 || M > F8_MAX || N < 1 || N > F8_MAX || K < 1 || K > F8_MAX || lda % 16 || ldw % 16) return -10;
   if (M == 0) return 0;
   Fp8Params p{};
   p.a_scales = a_scales; p.b_scales = b_scales; p.a_row = a_row; p.a_block = a_block; p.b_row = b_row; p.b_block = b_block;

@@ -663,7 +663,7 @@ bool rows8(const Tensor& t, const Tensor& scales, int64_t block_rows, const Tens
 
 Optional matmul_fp8(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, const Tensor& status) {
   if (!(a.is_cuda() && rows8(a, sa, 1, a) && rows8(b, sb, 128, a) && a.size(1) == b.size(1) &&
-        std::max({a.size(0), a.size(1), b.size(0)}) <= INT_MAX - 127))
+        std::max({a.size(0), a.size(1), b.size(0)}) <= INT_MAX - 255))
     return std::nullopt;
   const c10::cuda::CUDAGuard guard(a.device());
   Tensor out = bf16({a.size(0), b.size(0)}, a);
@@ -675,7 +675,7 @@ Optional matmul_fp8(const Tensor& a, const Tensor& sa, const Tensor& b, const Te
 Optional linear_fp8(const Tensor& x, const Tensor& weight, const Optional& values, const Optional& scales, const Tensor& status) {
   if (!(x.is_cuda() && x.dim() >= 1 && x.numel() > 0 && plain(x, at::kBFloat16, x) && weight.dim() == 2 && weight.size(0) > 0 &&
         x.size(-1) == weight.size(1) && weight.device() == x.device() &&
-        std::max({x.numel() / x.size(-1), weight.size(0), weight.size(1)}) <= INT_MAX - 127))
+        std::max({x.numel() / x.size(-1), weight.size(0), weight.size(1)}) <= INT_MAX - 255))
     return std::nullopt;
   const int64_t N = weight.size(0), K = weight.size(1);
   if (N % 8 || K % 32 || !(weight.scalar_type() == at::kBFloat16 || weight.scalar_type() == at::kFloat)) return std::nullopt;

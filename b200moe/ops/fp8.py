@@ -11,10 +11,12 @@ from torch.autograd.function import once_differentiable
 
 from . import backward_follows, cpp_nodes, functional as Fn, native, use_native
 
+MAX_SIZE = 2 ** 31 - 256         # rows and columns, which the kernels round up to whole tiles in 32 bits
+
 
 def _check_size(name: str, x) -> None:
-    if max(x.shape) > 2 ** 31 - 128:
-        raise ValueError(f"{name} {list(x.shape)} has more than 2^31 - 128 rows or columns")
+    if max(x.shape) > MAX_SIZE:
+        raise ValueError(f"{name} {list(x.shape)} has more than 2^31 - 256 rows or columns")
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1):
@@ -133,8 +135,8 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_fp8=None) -> torch.
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or min(weight.shape) < 1:
         raise ValueError(f"x {list(x.shape)} and weight {list(weight.shape)} must share their last dimension, and the weight have a row")
     _check_size("weight", weight)
-    if x.numel() // x.shape[-1] > 2 ** 31 - 128:
-        raise ValueError(f"x {list(x.shape)} has more than 2^31 - 128 rows")
+    if x.numel() // x.shape[-1] > MAX_SIZE:
+        raise ValueError(f"x {list(x.shape)} has more than 2^31 - 256 rows")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
     if getattr(weight, "pending_gather", None) is not None:

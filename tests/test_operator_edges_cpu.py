@@ -35,3 +35,27 @@ def test_gated_norm_refuses_rows_whose_counters_would_overflow(library):
             for rows in (2 ** 31 - 2 ** 16 + 1, 2 ** 31 - 2, 2 ** 31 - 1):
                 assert call(rows, D) == REFUSED
             assert call(2 ** 31 - 2 ** 16, D) != REFUSED
+
+
+def test_fp8_refuses_sizes_that_whole_tiles_round_up_beyond_32_bits(library):
+    null, large = P(None), 2 ** 31 - 255
+
+    def product(M, N, K):
+        return library.b2_gemm_fp8(*[null] * 5, I(M), I(N), I(K), *[L(16)] * 2, *[L(1)] * 4, I(0), null, null)
+
+    def quantize(M, K):
+        pitch = (K + 15) // 16 * 16
+        return library.b2_quantize_fp8(null, I(1), null, null, L(M), I(K), L(K), L(pitch), L(M), I(1), null)
+
+    for sizes in ((large, 1, 1), (1, large, 1), (1, 1, large), (1, 2 ** 31 - 128, 1)):
+        assert product(*sizes) == REFUSED
+    assert quantize(large, 1) == quantize(1, large) == REFUSED
+    from b200moe import ops
+    one = torch.zeros(1, 1, dtype=torch.bfloat16)
+    for shape in ((large, 1), (1, 2 ** 31 - 128)):
+        with pytest.raises(ValueError, match="rows or columns"):
+            ops.quantize_fp8(one.expand(shape))
+        with pytest.raises(ValueError, match="rows or columns"):
+            ops.linear_fp8(one.expand(1, shape[1]), one.expand(shape))
+    with pytest.raises(ValueError, match="rows"):
+        ops.linear_fp8(one.expand(large, 1), one)

@@ -60,6 +60,13 @@ def backward_follows(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def autograd_sees(*tensors) -> bool:
+    """Whether a call on ``tensors`` goes through its autograd function: a backward pass may follow, or forward-mode
+    differentiation is on, which asks for no gradient and refuses the function (a launch without it would drop the tangents)."""
+    from torch.autograd import forward_ad
+    return backward_follows(*tensors) or forward_ad._current_level >= 0
+
+
 from .dense import linear, linear_rope, swiglu_ffn, embedding, rmsnorm, add_rmsnorm, gated_add_rmsnorm  # noqa: E402
 from .attention import rope_attention  # noqa: E402
 from .loss import lm_head_cross_entropy  # noqa: E402

@@ -16,7 +16,7 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import backward_follows, cpp_nodes, functional as Fn, native, use_native
+from . import autograd_sees, backward_follows, cpp_nodes, functional as Fn, native, use_native
 
 
 class _Linear(torch.autograd.Function):
@@ -314,6 +314,6 @@ def gated_add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, delta_weight: torch.
         raise ValueError(f"at most 2^31 - 2^16 rows, got {x.numel() // width}")
     seq = x.numel() // max(x.shape[0] * width, 1) if kind == 2 else 1
     args = (x, delta, delta_weight, weight, gate, kind, max(seq, 1), float(residual_scale), float(eps))
-    if backward_follows(x, delta, delta_weight, weight, gate):
+    if autograd_sees(x, delta, delta_weight, weight, gate):
         return _GatedAddRMSNorm.apply(*args)
     return _gated_add_rmsnorm(*args)[:2]

@@ -26,7 +26,7 @@ import torch.distributed as dist
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
-from . import backward_follows, cpp_nodes, functional as Fn, native, use_native
+from . import autograd_sees, cpp_nodes, functional as Fn, native, use_native
 
 ALIGN = 128
 
@@ -118,7 +118,7 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: to
     if not use_native(logits, "route"):
         return Fn.route_topk_ref(logits, k, score, bias, groups, top_groups, group_score, renormalize, scale)
     how = (k, score == "sigmoid", bias, groups, top_groups, group_score == 2, bool(renormalize), float(scale))
-    if backward_follows(logits):
+    if autograd_sees(logits):
         return _RouteTopk.apply(logits.contiguous(), *how)
     return native.route_topk_fwd(logits.contiguous(), *how)
 

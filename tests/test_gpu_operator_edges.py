@@ -107,6 +107,25 @@ def test_renormalised_sigmoids_far_apart():
     assert bool(((got.double().cpu() - exact).abs() <= 256 * 2.0 ** -24 * size + 2.0 ** -146).all())
 
 
+# ------------------------------------------------------------------------------ differentiation forward
+def test_forward_mode_is_refused_and_not_dropped():
+    from torch.autograd import forward_ad
+    x, w = torch.randn(4, 64, device="cuda").bfloat16(), torch.ones(64, device="cuda")
+    logits = torch.randn(4, 64, device="cuda")
+    with forward_ad.dual_level():
+        for t in (x, logits, w):
+            dual = forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(RuntimeError):
+                if t is x:
+                    ops.gated_add_rmsnorm(dual, x, w, w)
+                elif t is w:
+                    ops.gated_add_rmsnorm(x, x, w, w, gate=dual)
+                else:
+                    ops.route_topk(dual, 3)
+        ops.gated_add_rmsnorm(x, x, w, w)               # plain operands are taken inside of a level too
+        ops.route_topk(logits, 3)
+
+
 # ------------------------------------------------------------------------------ sizes
 def test_gated_norm_refuses_rows_whose_counters_would_overflow():
     one, w = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16), torch.ones(1, device="cuda")

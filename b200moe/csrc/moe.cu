@@ -494,6 +494,7 @@ int b2_moe_gather(const void* x, const int* row_slot, const int* meta, const flo
 int b2_moe_combine(const void* y_perm, const int* slot_row, const float* weights, const void* residual, void* out,
                    int T, int D, int rows, cudaStream_t s) {
   if (D % 8) return -10;
+  if (T == 0) return 0;
   launch_next(moe_combine_kernel, min((T + 7) / 8, sm_count_moe() * 8), 256, 0, s, (const bf16*)y_perm, slot_row, weights,
               (const bf16*)residual, (bf16*)out, T, D, rows);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
@@ -503,6 +504,7 @@ int b2_moe_combine(const void* y_perm, const int* slot_row, const float* weights
 int b2_moe_combine_k(const void* y_perm, const int* slot_row, const float* weights, void* out, int T, int D, int rows, int k,
                      cudaStream_t s) {
   if (D % 8 || k < 1 || k > 32) return -10;
+  if (T == 0) return 0;
   launch_next(moe_combine_k_kernel, min((T + 7) / 8, sm_count_moe() * 8), 256, 0, s, (const bf16*)y_perm, slot_row, weights,
               (bf16*)out, T, D, rows, k);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;

@@ -148,3 +148,19 @@ def test_quantize_fp8_statement_on_the_gpu_is_that_on_the_cpu():
         assert torch.equal(scales.cpu(), s) and torch.equal(values.cpu().view(torch.uint8), v.view(torch.uint8))
         own = ops.quantize_fp8(x, block_rows)
         assert torch.equal(own[1], scales) and torch.equal(own[0].contiguous().view(torch.uint8), values.view(torch.uint8))
+
+
+# ------------------------------------------------------------------------------ no tokens
+@pytest.mark.parametrize("k", [1, 2, 3])
+def test_moe_ffn_of_no_tokens(k):
+    E, D, F = 8, 128, 256
+    x = torch.zeros(0, D, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    w1, w3 = (torch.randn(E, F, D, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    w2 = torch.randn(E, D, F, device="cuda").bfloat16().requires_grad_()
+    weights, idx = ops.route_topk(torch.zeros(0, E, device="cuda"), k)
+    weights.requires_grad_()
+    y = ops.moe_ffn(x, weights, idx, w1, w2, w3)
+    assert y.shape == (0, D) and y.dtype == torch.bfloat16
+    grads = torch.autograd.grad(y, (x, weights, w1, w2, w3), torch.empty_like(y))
+    assert grads[0].shape == (0, D) and grads[1].shape == (0, k) and all(g.shape == w.shape and not g.any() for g, w in
+                                                                          zip(grads[2:], (w1, w2, w3)))

@@ -311,13 +311,18 @@ def moe_ffn(x: torch.Tensor, weights: torch.Tensor, idx: torch.Tensor, w1, w2, w
             group=None, recompute: bool = False, budget=None) -> torch.Tensor:
     """Dispatch ``x [T, D]`` to its experts ``idx [T, k]``, run them, combine with ``weights``.  ``w1, w3: [E_local, d_ff,
     D]``, ``w2: [E_local, D, d_ff]``.  On one rank the kernels take up to 32 experts per token out of up to 1024."""
+    if x.dim() != 2 or idx.dim() != 2 or weights.shape != idx.shape or idx.shape[0] != x.shape[0]:
+        raise ValueError(f"x [T, D], weights [T, k] and idx [T, k] must belong together, got {list(x.shape)}, "
+                         f"{list(weights.shape)} and {list(idx.shape)}")
     tokens, k = idx.shape
     ep = 1 if group is None else dist.get_world_size(group)
     if use_native(x, "moe") and ep == 1:
         if not 1 <= k <= 32:
             raise ValueError(f"between 1 and 32 experts per token, got {k}")
+        if weights.device != x.device or idx.device != x.device:
+            raise ValueError(f"all tensors must be on {x.device}, got weights on {weights.device} and idx on {idx.device}")
         from .moe_fused import moe_ffn_fused
-        return moe_ffn_fused(x, weights, idx, w1, w2, w3, recompute=recompute, budget=budget)
+        return moe_ffn_fused(x, weights, idx.long(), w1, w2, w3, recompute=recompute, budget=budget)
     plan = build_plan(idx, w1.shape[0] * ep, group)
     sent = x[plan.order // k]
     received = sent if ep == 1 else _AllToAllRows.apply(sent, plan.send_splits, plan.recv_splits, group)

@@ -164,3 +164,16 @@ def test_moe_ffn_of_no_tokens(k):
     grads = torch.autograd.grad(y, (x, weights, w1, w2, w3), torch.empty_like(y))
     assert grads[0].shape == (0, D) and grads[1].shape == (0, k) and all(g.shape == w.shape and not g.any() for g, w in
                                                                           zip(grads[2:], (w1, w2, w3)))
+
+
+def test_moe_ffn_looks_at_its_operands():
+    E, D, F, T = 8, 128, 256, 40
+    x = torch.randn(T, D, device="cuda").bfloat16()
+    experts = [torch.randn(E, *shape, device="cuda").bfloat16() for shape in ((F, D), (D, F), (F, D))]
+    weights, idx = ops.route_topk(torch.randn(T, E, device="cuda"), 3)
+    y = ops.moe_ffn(x, weights, idx, *experts)
+    assert torch.equal(ops.moe_ffn(x, weights, idx.int(), *experts), y)       # the kernels read 64-bit indices
+    for bad in ((x, weights[:, :1], idx), (x[:39], weights, idx), (x, weights[:39], idx[:39]), (x, weights.cpu(), idx),
+                (x, weights, idx.cpu())):
+        with pytest.raises(ValueError):
+            ops.moe_ffn(*bad, *experts)

@@ -59,3 +59,14 @@ def test_fp8_refuses_sizes_that_whole_tiles_round_up_beyond_32_bits(library):
             ops.linear_fp8(one.expand(1, shape[1]), one.expand(shape))
     with pytest.raises(ValueError, match="rows"):
         ops.linear_fp8(one.expand(large, 1), one)
+
+
+def test_moe_ffn_refuses_operands_that_do_not_belong_together():
+    from b200moe import ops
+    x, experts = torch.randn(5, 16), [torch.randn(4, 24, 16), torch.randn(4, 16, 24), torch.randn(4, 24, 16)]
+    weights, idx = ops.route_topk(torch.randn(5, 4), 3)
+    assert ops.moe_ffn(x, weights, idx, *experts).shape == (5, 16)
+    for bad in ((x, weights[:, :1], idx), (x, weights, idx[:, :2]), (x[:4], weights, idx), (x, weights[:4], idx[:4]),
+                (x, weights.flatten(), idx.flatten()), (x[None], weights, idx)):
+        with pytest.raises(ValueError, match="belong together"):
+            ops.moe_ffn(*bad, *experts)

@@ -14,6 +14,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
+#include <cmath>
 
 #include "entries.h"
 
@@ -609,8 +611,8 @@ std::optional<variable_list> route_topk(const Tensor& logits, const Optional& bi
     return std::nullopt;
   const int64_t E = logits.size(1);
   if (!(E >= 1 && E <= 1024 && groups >= 1 && groups <= 32 && E % groups == 0 && top_groups >= 1 && top_groups <= groups && k >= 1 &&
-        k <= 32 && k <= E / groups * top_groups && (group_score == 1 || (group_score == 2 && E / groups >= 2)) && std::isfinite(scale) &&
-        scale != 0.0))
+        k <= 32 && k <= E / groups * top_groups && (group_score == 1 || (group_score == 2 && E / groups >= 2)) &&
+        std::fabs(scale) >= FLT_MIN && std::fabs(scale) <= FLT_MAX))
     return std::nullopt;
   if (bias && !(bias->dim() == 1 && bias->size(0) == E && bias->scalar_type() == at::kFloat && bias->is_contiguous() &&
                 bias->device() == logits.device() && !bias->requires_grad()))
@@ -623,7 +625,8 @@ std::optional<variable_list> gated_norm(const Tensor& x, const Tensor& delta, co
                                         double scale, double eps, const Tensor& status) {
   const int64_t dims = x.dim();
   if (!(x.is_cuda() && dims >= 1 && x.numel() > 0 && float_type(x) >= 0 && x.is_contiguous() && delta.sizes() == x.sizes() &&
-        delta.scalar_type() == x.scalar_type() && delta.is_contiguous() && delta.device() == x.device() && std::isfinite(scale) && eps > 0))
+        delta.scalar_type() == x.scalar_type() && delta.is_contiguous() && delta.device() == x.device() && std::fabs(scale) <= FLT_MAX &&
+        eps >= FLT_MIN && eps <= FLT_MAX))
     return std::nullopt;
   const int64_t D = x.size(-1);
   if (!(D <= 8192 && x.numel() / D <= INT_MAX - 0xffff)) return std::nullopt;

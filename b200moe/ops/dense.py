@@ -11,8 +11,6 @@ Replaces the reference's ``einsum`` linear (implementation/layers.py:55-69),
 """
 from __future__ import annotations
 
-import math
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -301,8 +299,8 @@ def gated_add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, delta_weight: torch.
     if x.dtype != delta.dtype or (gate is not None and gate.dtype not in (x.dtype, torch.float32)):
         raise TypeError(f"x and delta must have one type, the gate that or fp32: got {x.dtype}, {delta.dtype}"
                         f"{'' if gate is None else f', {gate.dtype}'}")
-    if not (math.isfinite(residual_scale) and eps > 0):
-        raise ValueError(f"residual_scale must be finite and eps positive, got {residual_scale} and {eps}")
+    if not (abs(residual_scale) <= Fn.FLT_MAX and Fn.FLT_MIN <= eps <= Fn.FLT_MAX):
+        raise ValueError(f"residual_scale must be finite and eps positive in fp32, got {residual_scale} and {eps}")
     for t in (delta, delta_weight, weight, gate):
         if t is not None and t.device != x.device:
             raise ValueError(f"all tensors must be on {x.device}, got one on {t.device}")

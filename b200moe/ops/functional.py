@@ -136,6 +136,9 @@ def router_top2_ref(logits: torch.Tensor, k: int = 2):
     return top / top.sum(dim=-1, keepdim=True), idx
 
 
+FLT_MIN, FLT_MAX = 2.0 ** -126, torch.finfo(torch.float32).max       # of the numbers that kernels take in fp32
+
+
 def route_topk_ref(logits: torch.Tensor, k: int, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
                    top_groups: int | None = None, group_score: int = 1, renormalize: bool = True, scale: float = 1.0):
     """``(weights fp32 [T, k], idx int64 [T, k])`` of ``logits [T, E]``.  Experts are chosen by their scores plus ``bias``
@@ -146,7 +149,7 @@ def route_topk_ref(logits: torch.Tensor, k: int, score: str = "softmax", bias: t
     tokens, experts = logits.shape
     top_groups = groups if top_groups is None else top_groups
     wide = logits if logits.dtype == torch.float64 else logits.float()
-    x = torch.where(torch.isnan(wide), -math.inf, wide).clamp(max=torch.finfo(torch.float32).max)
+    x = torch.where(torch.isnan(wide), -math.inf, wide).clamp(max=FLT_MAX)
     dead = torch.isinf(x)
 
     def scores(t, off):

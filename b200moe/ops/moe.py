@@ -18,7 +18,6 @@ tier and the NCCL A/B baseline.
 """
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -109,8 +108,8 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: to
         raise ValueError(f"at most 1024 experts, got {experts}")
     if group_score not in (1, 2) or (group_score == 2 and experts // groups < 2):
         raise ValueError(f"group_score must be 1 or, for groups of two experts or more, 2, got {group_score}")
-    if not (math.isfinite(scale) and scale != 0):
-        raise ValueError(f"scale must be finite and not zero, got {scale}")
+    if not Fn.FLT_MIN <= abs(scale) <= Fn.FLT_MAX:
+        raise ValueError(f"scale must be finite and not zero in fp32, got {scale}")
     if bias is not None:
         if bias.shape != (experts,) or bias.device != logits.device:
             raise ValueError(f"bias must be [{experts}] on {logits.device}, got {tuple(bias.shape)} on {bias.device}")

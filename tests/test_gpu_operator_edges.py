@@ -138,6 +138,20 @@ def test_gated_norm_refuses_rows_whose_counters_would_overflow():
             ops.gated_add_rmsnorm(many, many, w, w)
 
 
+def test_factors_are_numbers_of_fp32():
+    x, w = torch.randn(3, 8, device="cuda"), torch.ones(8, device="cuda")
+    for bad in (1e300, -1e39):
+        with pytest.raises(ValueError, match="scale"):
+            ops.route_topk(x, 2, scale=bad)
+        with pytest.raises(ValueError, match="residual_scale"):
+            ops.gated_add_rmsnorm(x, x, w, w, residual_scale=bad)
+    for bad in (1e-60, 1e300):
+        with pytest.raises(ValueError, match="eps"):
+            ops.gated_add_rmsnorm(x, x, w, w, eps=bad)
+    with pytest.raises(ValueError, match="scale"):
+        ops.route_topk(x, 2, scale=1e-60)
+
+
 # ------------------------------------------------------------------------------ 8-bit values
 def test_quantize_fp8_statement_on_the_gpu_is_that_on_the_cpu():
     from b200moe.ops import functional as Fn

@@ -1,5 +1,6 @@
 """Routing, gated residual norm and 8-bit products: sizes and operands at the edge of what they take."""
 import ctypes
+import math
 import os
 
 import pytest
@@ -70,3 +71,21 @@ def test_moe_ffn_refuses_operands_that_do_not_belong_together():
                 (x, weights.flatten(), idx.flatten()), (x[None], weights, idx)):
         with pytest.raises(ValueError, match="belong together"):
             ops.moe_ffn(*bad, *experts)
+
+
+FACTORS = [1e300, -1e39, math.inf, math.nan]             # none of them is a number of fp32
+
+
+def test_factors_are_numbers_of_fp32():
+    from b200moe import ops
+    x, w = torch.randn(3, 8), torch.ones(8)
+    for bad in FACTORS + [0.0, 1e-60]:
+        with pytest.raises(ValueError, match="scale"):
+            ops.route_topk(x, 2, scale=bad)
+    for bad in FACTORS:
+        with pytest.raises(ValueError, match="residual_scale"):
+            ops.gated_add_rmsnorm(x, x, w, w, residual_scale=bad)
+    for bad in FACTORS + [0.0, 1e-60, -1e-5]:
+        with pytest.raises(ValueError, match="eps"):
+            ops.gated_add_rmsnorm(x, x, w, w, eps=bad)
+    assert ops.gated_add_rmsnorm(x, x, w, w, residual_scale=0.0)[0].shape == x.shape

@@ -50,9 +50,9 @@ struct GatedNormParams {
   void* dx;
   void* ddelta;
   void* dgate;               // [rows] or [rows, D] (GATE_TOKEN, GATE_FULL)
-  float* partial;            // [2][CTAs][D] column sums, then for GATE_SEQUENCE [CTAs + sequences][rows at a time][D]
+  float* partial;            // [2][CTAs][D] column sums, then for GATE_SEQUENCE [CTAs + sequences][places][D]
   int* status;               // device word, non-zero: a wait ran out
-  int rows, D, seq, gate_kind, gate_f32, aligned, stages, ctas_per_sm;
+  int rows, D, seq, places, gate_kind, gate_f32, aligned, stages, ctas_per_sm;
   float residual_scale, eps;
 };
 
@@ -265,6 +265,15 @@ static int gn_sms() {
 }
 
 static int gn_rows_at_once(int D) { return D <= 512 ? 8 : D <= 1024 ? 4 : D <= 2048 ? 2 : 1; }
+
+// Sums of a sequence in a CTA, one for each of its slots, or as many as the sequence has rows (the next power of two), which lie in slots one
+// after the other.
+static int gn_places(int D, int seq) {
+  const int R = gn_rows_at_once(D);
+  int n = 1;
+  while (n < R && n < seq) n *= 2;
+  return n;
+}
 
 // CTAs of the backward kernels: ``per_sm`` of them, at least two blocks of rows each, so that the partial sums stay small beside the
 // rows.

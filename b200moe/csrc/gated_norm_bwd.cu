@@ -37,7 +37,7 @@ __device__ __forceinline__ void gn_store_sums(const GatedNormParams& p, float (&
 
 // Column sums stay in registers while a worker goes through its rows: dw and, where a gate of its own has no column sum, dw_d.
 // With a gate that rows share the sum a = sum of dS nhat gives both its gradient, w_d a, and dw_d, g a; for a gate per sequence a
-// is stored wherever the sequence changes, in place ``sequence + CTA`` and slot, which no other has.
+// is stored wherever the sequence changes, in place ``sequence + CTA`` and slot (of as many as the sequence can use), which no other has.
 template <typename T, int W, int GATE>       // GATE: 0 no column sums, 1 a gate per channel, 2 a gate per sequence
 __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const GatedNormParams p) {
   chain_begin();
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(gn_threads<W>()) gated_norm_bwd_kernel(const G
       e.store(static_cast<T*>(p.ddelta) + at, col, D, p.aligned);
     }
     if (GATE == 2 && (row + R >= end || row / p.seq != (row + R) / p.seq)) {
-      float* dst = sequences + (static_cast<long long>(row / p.seq + blockIdx.x) * R + slot) * D;
+      float* dst = sequences + (static_cast<long long>(row / p.seq + blockIdx.x) * p.places + (slot & p.places - 1)) * D;
 #pragma unroll
       for (int c = 0; c < V; ++c) {
         const int col = ((c * W + in_row) * 32 + lane) * 8;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(gn_threads<W>(), W == 16 ? 1 : 2) gated_norm_b
       e.store(static_cast<T*>(p.ddelta) + at, col, D, true);
     }
     if (G == GATE_SEQUENCE && row + R >= min(end, sequence_end)) {
-      float* dst = sequences + (static_cast<long long>(sequence + blockIdx.x) * R + slot) * D;
+      float* dst = sequences + (static_cast<long long>(sequence + blockIdx.x) * p.places + (slot & p.places - 1)) * D;
 #pragma unroll
       for (int c = 0; c < V; ++c) {
         const int col = ((c * W + in_row) * 32 + lane) * 8;
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(gn_threads<W>(), W == 16 ? 1 : 2) gated_norm_b
 // Column sums of the partial rows: VEC columns a thread, 16 partial rows at a time.  blockIdx.y: 0 dw; 1 dw_d, and the gradient of a
 // gate per channel; 2 + i the gradient of sequence i's gate.
 template <int VEC>
-__global__ void __launch_bounds__(512) gated_norm_sums_kernel(const GatedNormParams p, int ctas, int per_cta, int gate_bf16,
+__global__ void __launch_bounds__(512) gated_norm_sums_kernel(const GatedNormParams p, int ctas, int gate_bf16,
                                                               float* __restrict__ dw, float* __restrict__ dwd,
                                                               void* __restrict__ dgate) {
   chain_begin();
@@ -415,13 +415,13 @@ __global__ void __launch_bounds__(512) gated_norm_sums_kernel(const GatedNormPar
       const int i = static_cast<int>(what - 2), low = i * p.seq, high = low + p.seq;
       const int first = gn_cta_of(low, p.rows, ctas), last = gn_cta_of(high - 1, p.rows, ctas) + 1;
       const int base = p.rows / ctas, extra = p.rows % ctas;           // as gn_first_row
-      const float* src = p.partial + (2LL * ctas + static_cast<long long>(i) * per_cta) * D + col;
-      const int shift = 31 - __clz(per_cta);                           // a power of two
+      const float* src = p.partial + (2LL * ctas + static_cast<long long>(i) * p.places) * D + col;
+      const int shift = 31 - __clz(p.places);                           // a power of two
       for (int r = (first << shift) + threadIdx.y; r < last << shift; r += 16) {
         // a slot that had none of the sequence's rows in this CTA has stored nothing
         const int cta = r >> shift, begin = cta * base + min(cta, extra), end = begin + base + (cta < extra);
         const int from = max(low, begin), rows = min(high, end) - from;
-        if ((r - (from - begin) & per_cta - 1) < rows) add(sum, src + static_cast<long long>(r) * D);
+        if ((r - (from - begin) & p.places - 1) < rows) add(sum, src + static_cast<long long>(r) * D);
       }
     }
     __syncthreads();
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(512) gated_norm_sums_kernel(const GatedNormPar
 
 template <typename T, int W>
 static cudaError_t gn_backward(GatedNormParams& p, int type, float* dw, float* dwd, cudaStream_t s) {
-  constexpr int R = gn_rows<W>(), THREADS = gn_threads<W>();
+  constexpr int THREADS = gn_threads<W>();
   const int ctas = gn_bwd_ctas(p.rows, p.D, W == 16 ? 1 : 2), gate_bf16 = type == 1;
   uint32_t smem;
   cudaError_t r;
@@ -481,8 +481,8 @@ static cudaError_t gn_backward(GatedNormParams& p, int type, float* dw, float* d
   const long long sums = 2 + (p.gate_kind == GATE_SEQUENCE ? p.rows / p.seq : 0);
   const unsigned y = static_cast<unsigned>(sums < 32768 ? sums : 32768);
   if (p.aligned)
-    return launch_next(gated_norm_sums_kernel<4>, dim3((p.D + 127) / 128, y), dim3(32, 16), 0, s, p, ctas, R, gate_bf16, dw, dwd, p.dgate);
-  return launch_next(gated_norm_sums_kernel<1>, dim3((p.D + 31) / 32, y), dim3(32, 16), 0, s, p, ctas, R, gate_bf16, dw, dwd, p.dgate);
+    return launch_next(gated_norm_sums_kernel<4>, dim3((p.D + 127) / 128, y), dim3(32, 16), 0, s, p, ctas, gate_bf16, dw, dwd, p.dgate);
+  return launch_next(gated_norm_sums_kernel<1>, dim3((p.D + 31) / 32, y), dim3(32, 16), 0, s, p, ctas, gate_bf16, dw, dwd, p.dgate);
 }
 
 }  // namespace b2
@@ -495,7 +495,7 @@ extern "C" {
 long long b2_gated_norm_bwd_floats(int rows, int D, int seq, int gate_kind) {
   if (rows < 1 || D < 1 || D > GN_MAX_D || (gate_kind == GATE_SEQUENCE && seq < 1)) return 0;
   const long long ctas = gn_bwd_ctas(rows, D, D <= 5120 ? 2 : 1);
-  return (2 * ctas + (gate_kind == GATE_SEQUENCE ? (ctas + rows / seq) * gn_rows_at_once(D) : 0)) * D;
+  return (2 * ctas + (gate_kind == GATE_SEQUENCE ? (ctas + rows / seq) * gn_places(D, seq) : 0)) * D;
 }
 
 // Gradients; dsummed and dnormed may be null (zero).  dgate has the gate's shape and type; dw, dwd fp32 [D].
@@ -506,7 +506,7 @@ int b2_gated_norm_bwd(const void* dsummed, const void* dnormed, const void* x, c
   GatedNormParams p{};
   p.x = x; p.delta = delta; p.delta_weight = delta_weight; p.weight = weight; p.gate = gate;
   p.delta_rstd = const_cast<float*>(delta_rstd); p.rstd = const_cast<float*>(rstd); p.dsummed = dsummed; p.dnormed = dnormed;
-  p.dx = dx; p.ddelta = ddelta; p.dgate = dgate; p.partial = partial; p.rows = rows; p.D = D; p.seq = seq;
+  p.dx = dx; p.ddelta = ddelta; p.dgate = dgate; p.partial = partial; p.rows = rows; p.D = D; p.seq = seq; p.places = gn_places(D, seq);
   p.gate_kind = gate_kind; p.gate_f32 = gate_f32; p.residual_scale = residual_scale; p.status = status;
   return gated_norm<true>(p, type, [&](auto tag, auto width) { return gn_backward<decltype(tag), decltype(width)::value>(p, type, dw, dwd, s); });
 }

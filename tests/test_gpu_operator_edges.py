@@ -152,6 +152,14 @@ def test_factors_are_numbers_of_fp32():
         ops.route_topk(x, 2, scale=1e-60)
 
 
+@pytest.mark.parametrize("B,S,D", [(1500, 2, 512), (900, 3, 264), (700, 7, 128), (1300, 4, 1000), (800, 9, 512), (601, 2, 1024), (301, 5, 2048),
+                                   (40, 3, 100), (6, 2, 1999), (5001, 2, 64)])
+def test_gated_norm_of_short_sequences(B, S, D):
+    from test_gpu_operators import _check_norm, _norm_case
+    for dtype in (torch.bfloat16, torch.float32):
+        _check_norm(*_norm_case(B, S, D, "sequence", dtype))
+
+
 # ------------------------------------------------------------------------------ 8-bit values
 def test_quantize_fp8_statement_on_the_gpu_is_that_on_the_cpu():
     from b200moe.ops import functional as Fn

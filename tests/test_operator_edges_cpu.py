@@ -38,6 +38,17 @@ def test_gated_norm_refuses_rows_whose_counters_would_overflow(library):
             assert call(2 ** 31 - 2 ** 16, D) != REFUSED
 
 
+def test_gated_norm_workspace_is_no_larger_than_the_tensor_for_short_sequences(library):
+    library.b2_gated_norm_bwd_floats.restype = L
+    rows = 2 ** 20 * 3
+    for D in (64, 512, 1024, 4096):
+        for seq in (2, 3, 4, 6, 8, 16, 512):
+            per_sequence = library.b2_gated_norm_bwd_floats(I(rows), I(D), I(seq), I(2))
+            assert 0 < per_sequence - library.b2_gated_norm_bwd_floats(I(rows), I(D), I(seq), I(1)) < 2 * rows * D
+            if seq & (seq - 1) == 0:
+                assert per_sequence <= rows * D
+
+
 def test_fp8_refuses_sizes_that_whole_tiles_round_up_beyond_32_bits(library):
     null, large = P(None), 2 ** 31 - 255
 

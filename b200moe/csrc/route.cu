@@ -311,8 +311,10 @@ __device__ __forceinline__ int choose(const RouteParams& p, long long row, const
       const float reach = value == -INFINITY ? 0.f : fmaxf(fabsf(best), p.two_best && second != -INFINITY ? fabsf(second) : 0.f);
       const float error = (p.two_best ? 2.f : 1.f) * key_error(most, 3.f * reach, p.sigmoid);
       const bool stays = group && in_front < p.top_groups, goes = group && !stays && value != -INFINITY;
-      const float low = row_max_f<LANES>(stays ? error - value : -INFINITY), high = row_max_f<LANES>(goes ? value + error : -INFINITY);
-      close = high != -INFINITY && !(-low > high);
+      // (a value that overflowed has no lower bound)
+      const uint32_t low = __reduce_min_sync(ALL, stays ? ordered(fmaxf(value - error, -INFINITY)) : ALL);
+      const uint32_t high = __reduce_max_sync(ALL, goes ? ordered(value + error) : 0u);
+      close = low <= high;
     }
   }
   // Without a bias experts are compared by their logits, whatever the groups were compared by.
@@ -408,10 +410,11 @@ __device__ __forceinline__ int choose(const RouteParams& p, long long row, const
     // the run that leaves the first k between their last pair and the one behind it
     const bool leaves = p.k < LANES && (nears >> (p.k - 1) & nears >> p.k & 1);
     close |= doubtful && !alone && (lane < p.k || (lane == p.k && leaves));
-    if (__any_sync(ALL, leaves && steps < candidates)) {      // it may go on behind the last key that was looked at
+    const bool beyond = leaves && steps < candidates;
+    if (LANES == 32 ? beyond : __any_sync(ALL, beyond)) {      // it may go on behind the last key that was looked at
       const float next = unordered(row_max<LANES>(h[0]));
       const float last = unordered(__shfl_sync(ALL, my_key, min(steps - 1, LANES - 1), LANES));
-      close |= leaves && steps < candidates && next != -INFINITY &&
+      close |= beyond && next != -INFINITY &&
                last - next <= key_error(most, last, p.sigmoid) + key_error(most, next, p.sigmoid);
     }
     const unsigned swaps = row_ballot<LANES>(swap);
@@ -557,9 +560,14 @@ __global__ void __launch_bounds__(route_warps(V) * 32, 4) route_fwd_kernel(const
   if (p.renormalize) {
     // Softmax: the other experts cancel.  Sigmoids of negative logits are exp(x) / (1 + exp(x)), all over exp(top) where none is positive: a
     // score that fp32 does not hold may have a weight that it does.
-    const float top = row_max_f<LANES>(xe), off = p.sigmoid ? fminf(top, 0.f) : top;
-    w = xe == -INFINITY ? 0.f : expf((p.sigmoid ? fminf(xe, 0.f) : xe) - off);
-    if (p.sigmoid) w /= 1.f + expf(-fabsf(xe));
+    const float top = row_max_f<LANES>(xe);
+    if (p.sigmoid) {
+      const float small = expf(-fabsf(xe));
+      w = xe > 0.f ? 1.f : top < 0.f ? expf(xe - top) : small;
+      w = xe == -INFINITY ? 0.f : w / (1.f + small);
+    } else {
+      w = xe == -INFINITY ? 0.f : expf(xe - top);
+    }
     const float total = row_add<LANES>(w);
     w = total == 0.f ? 0.f : w / total;
   } else {

@@ -53,7 +53,7 @@ int b2_scale_bf16(void* x, const float* factor, long long n, cudaStream_t s);
 int b2_embedding_fwd(const long long* ids, const void* table, void* out, int T, int D, cudaStream_t s);
 int b2_embedding_bwd(const long long* ids, const void* dy, float* dtable, int T, int D, cudaStream_t s);
 int b2_moe_aux(const float* probs, const int* counts, float* aux, int T, int E, cudaStream_t s);
-// route.cu, gated_norm.cu, fp8.cu
+// route.cu, gated_norm_fwd.cu, gated_norm_bwd.cu, fp8.cu
 int b2_route_topk(const void* logits, const float* bias, float* weights, long long* idx, long long T, int E, int k, int type,
                   int sigmoid, int groups, int top_groups, int two_best, int renormalize, float scale, cudaStream_t s);
 int b2_route_topk_bwd(const void* logits, const float* weights, const long long* idx, const float* dweights, void* dlogits,

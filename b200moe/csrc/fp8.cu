@@ -13,9 +13,10 @@
 // epilogue multiply it by the two scales, which two warps form ahead, and add it to fp32 registers, while the next blocks are in
 // flight: accumulators of 512 / BN blocks fit in tensor memory.  A block of a 128 x 256 tile is 768 cycles of shared memory (48 KiB
 // written by TMA and read by the tensor cores, which would need 512), and one fused multiply-add per value, 256 issue slots of each
-// scheduler.  Large products run against the power limit: 16384 x 6144, K 4096 takes 408 us (2.0 PFLOP/s, bf16 520 us), without the
-// additions 320 us at a lower clock.  Pairs of CTAs (cta_group::2), which halve the traffic of B, were slower (616 us): an accumulator
-// goes back and forth between two CTAs for every block.
+// scheduler.  16384 x 6144, K 4096 takes 413 us in a launch by itself (2.0 PFLOP/s, bf16 520 us) and 482 in a loop, against the power limit
+// at 1.5 GHz.  The tensor cores are busy half of the cycles either way, and no unit is near its limit: what waits is the epilogue, which
+// loads columns, waits for them and adds them in turn (without the additions 320 us, three quarters of the cycles).  Pairs of CTAs
+// (cta_group::2), which halve the traffic of B, were slower (616 us): an accumulator goes back and forth between two CTAs for every block.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -117,7 +118,8 @@ __device__ __forceinline__ float largest8(const Values8<T>& x) {
 }
 
 // One scale for 128 values of a row: eight lanes per block with 8 values of each half of it; a CTA has 64 consecutive blocks, 32
-// where there are few.  ``pitch`` is a multiple of 16 and the row is filled with zeros up to it.  Bound by memory traffic.
+// where there are few.  ``pitch`` is a multiple of 16 and the row is filled with zeros up to it.  Bound by instructions, which are
+// issued in 72 % of the cycles where memory is at 48 % of its peak: 16384 x 4096 bf16 values take 43 us.
 template <typename T, int AHEAD>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                             float* __restrict__ scales, int M, int K, long long ldx,
@@ -159,8 +161,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 }
 
 // One scale for 128 x 128 values, 32 of them a thread: two CTAs per SM take the blocks in turn, and the next block is on its way while
-// the present one's largest value is found.  Bound by memory traffic: 16384 x 4096 bf16 values take 47 us, 4.3 TB/s; 76 with a CTA
-// for each block, whose loads stop while it waits for its maximum.
+// the present one's largest value is found.  Bound by instructions as the kernel above (78 %, memory at 46 %): 16384 x 4096 bf16 values
+// take 43 us; 76 with a CTA for each block, whose loads stop while it waits for its maximum.
 template <typename T>
 __global__ void __launch_bounds__(512, 2) quantize_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                                  float* __restrict__ scales, int M, int K, long long ldx,

@@ -718,8 +718,8 @@ static int route(const RouteParams& p, const float* dweights, void* dlogits, cud
     return launch_route_bwd<32, 32>(p, dweights, dlogits, s);
   }
   // Eight lanes per token where they hold the logits and have a lane per chosen expert: 65536 tokens, 6 of 64 experts 20 us (a warp
-  // per token: 33), backward 16 (25).  Sixteen lanes for up to 256 experts lose what they save: at 32768 tokens, 8 of
-  // 256 in groups with a bias, they took 58 us where a warp per token took 55 (now 40), though they issue a fifth fewer instructions.
+  // per token: 33), backward 10.  Sixteen lanes for up to 256 experts lose what they save: at 32768 tokens, 8 of
+  // 256 in groups with a bias, they took 58 us where a warp per token took 55 (now 46), though they issue a fifth fewer instructions.
   if (p.E <= 64 && p.k <= 8 && p.top_groups == p.groups) {
     if (p.E <= 8) return launch_route<8, 1>(p, s);
     if (p.E <= 16) return launch_route<8, 2>(p, s);

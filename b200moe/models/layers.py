@@ -264,9 +264,10 @@ class MoELayerMulti(nn.Module):
 
     ``routing``: keyword arguments of ``ops.route_topk`` (``score``, ``groups``, ``top_groups``, ``group_score``,
     ``renormalize``, ``scale``; an empty dict takes its defaults) for another router than the softmax of two experts, with
-    any ``k`` that it takes; ``balance_bias: True`` adds the buffer ``expert_bias``, which takes part in the choice and which
-    the training loop moves against the experts' load.  On a GPU the router's product has up to 16 experts or a multiple
-    of 64."""
+    any ``k`` that it takes; ``balance_bias: True`` adds the buffer ``expert_bias``, zeros, which takes part in the choice: a
+    program that balances by it moves it against the experts' load between its steps (the trainer does not).  On a GPU the
+    router's product has up to 16 experts or a multiple of 64.  On several ranks such a layer takes the exchange of
+    ``ops.moe``, not the one that is fused with the experts' products."""
 
     def __init__(self, d_model, d_ff, k=2, num_expert_per_node=4, device=None, dtype=torch.bfloat16,
                  dp_group=None, routing=None):

@@ -463,7 +463,7 @@ def rmsnorm_bwd(dy, x, weight, rstd, residual_grad=None):
 
 def gated_norm_fwd(x, delta, delta_weight, weight, gate, kind: int, seq: int, residual_scale: float, eps: float):
     """``x, delta [..., D]`` contiguous -> ``(summed, normed, stats)``, the latter 1 / rms of delta and of the sum; ``kind`` of
-    gate and layouts as in ``csrc/gated_norm.cu``."""
+    gate and layouts as in ``csrc/gated_norm.cuh``."""
     D = x.shape[-1]
     rows = x.numel() // D
     summed, normed = torch.empty_like(x), torch.empty_like(x)

@@ -11,7 +11,7 @@
 //
 // Bound by integer minima, comparisons and selections, which the ALU issues every other cycle, beyond 100 experts.
 //
-// The choice is that of exact arithmetic.  Comparisons of logits are exact as they are.  Comparisons of scores (a bias, a
+// The choice is that of 64-bit arithmetic.  Comparisons of logits are exact as they are.  Comparisons of scores (a bias, a
 // sum of two) are made in fp32 with the fast exponential and division first, and those that decided something are checked
 // against a bound on the error of both sides; a row in which one is closer than that is worked out again in 64 bits, by a whole
 // warp, plainly.

@@ -84,7 +84,8 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: to
     ``scale``         factor of the weights
 
     Experts come best first, the lower index first where two are equal; without a bias they are compared by their logits.  The
-    choice is that of exact arithmetic: scores that are too close for fp32 are compared in fp64.  A logit of -inf (or NaN)
+    choice is that of 64-bit arithmetic: scores that are too close for fp32 are compared in fp64 (sums of two scores with biases
+    of both signs that are equal but for fp64's own rounding go either way).  A logit of -inf (or NaN)
     masks an expert: it comes after all others of the chosen groups, with weight 0; +inf counts as the largest number."""
     if use_native(logits, "route"):
         nodes = cpp_nodes(logits) if bias is None else cpp_nodes(logits, bias)
